@@ -43,6 +43,11 @@ EXPORTED_SYMBOLS = (
     "feather_unprepack_bytes",
     "feather_dequantize",
     "feather_bf16_to_fp16",
+    "feather_mxfp4_scale_bytes",
+    "feather_mxfp4_quantize",
+    "feather_mxfp4_dequantize",
+    "feather_mxfp4_mm",
+    "feather_gated_norm",
     "feather_last_error_string",
     "feather_version",
 )
@@ -63,6 +68,18 @@ class MMVariant(ctypes.Structure):
 
     def as_tuple(self):
         return (self.tokens_tile, self.cta_pair, self.split_k, self.transform_groups, self.max_ctas, self.kernel, self.staging)
+
+
+class NormArgs(ctypes.Structure):
+    """Mirror of `feather_norm_args`."""
+
+    _fields_ = (
+        [(name, ctypes.c_void_p) for name in ("x", "y", "r", "h", "h_scales", "weight", "bias", "post_weight", "gate", "scale", "shift")]
+        + [(name, ctypes.c_int64) for name in ("rows", "cols", "ldx", "ldy", "ldr", "ldh", "gate_ld", "scale_ld", "shift_ld", "gate_rows", "scale_rows", "shift_rows")]
+        + [(name, ctypes.c_float) for name in ("residual_scale", "eps")]
+        + [(name, ctypes.c_int) for name in ("kind", "post_norm", "x_dtype", "y_dtype", "h_dtype", "weight_dtype", "bias_dtype", "post_weight_dtype",
+                                             "gate_dtype", "scale_dtype", "shift_dtype")]
+    )
 
 
 class FeatherNativeError(RuntimeError):
@@ -122,6 +139,16 @@ def load_library():
         lib.feather_dequantize.restype = ci
         lib.feather_bf16_to_fp16.argtypes = [vp, vp, i64, vp]
         lib.feather_bf16_to_fp16.restype = ci
+        lib.feather_mxfp4_scale_bytes.argtypes = [i64, i64]
+        lib.feather_mxfp4_scale_bytes.restype = sz
+        lib.feather_mxfp4_quantize.argtypes = [vp, ci, i64, i64, i64, vp, vp, vp]
+        lib.feather_mxfp4_quantize.restype = ci
+        lib.feather_mxfp4_dequantize.argtypes = [vp, vp, i64, i64, ci, vp, vp]
+        lib.feather_mxfp4_dequantize.restype = ci
+        lib.feather_mxfp4_mm.argtypes = [vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, ci, vp, vp]
+        lib.feather_mxfp4_mm.restype = ci
+        lib.feather_gated_norm.argtypes = [ctypes.POINTER(NormArgs), vp]
+        lib.feather_gated_norm.restype = ci
         lib.feather_last_error_string.argtypes = []
         lib.feather_last_error_string.restype = ctypes.c_char_p
         lib.feather_version.argtypes = []
@@ -605,3 +632,56 @@ def bf16_to_fp16(x):
         status = lib.feather_bf16_to_fp16(_ptr(x), _ptr(out), x.numel(), _stream_ptr(dev))
     _check(status, "feather_bf16_to_fp16")
     return out
+
+
+# ------------------------------------------------------------------------------------------------
+# MXFP4 and the fused norm
+# ------------------------------------------------------------------------------------------------
+def mxfp4_quantize_into(x, data, scales):
+    """x [R, K] fp32 / bf16 / fp16 with unit column stride -> data [R, K/2], scales [ceil(R/128), ceil(K/128), 512] (uint8, contiguous)."""
+    lib = load_library()
+    dev = _require_cuda(x, data, scales)
+    rows, k = x.shape
+    index = dev.index
+    with _OnDevice(index):
+        status = lib.feather_mxfp4_quantize(x.data_ptr(), _SRC_CODE[x.dtype], rows, k, x.stride(0), data.data_ptr(), scales.data_ptr(), _raw_stream(index))
+    if status != FEATHER_OK:
+        _check(status, "feather_mxfp4_quantize")
+
+
+def mxfp4_dequantize_into(data, scales, out):
+    lib = load_library()
+    dev = _require_cuda(data, scales, out)
+    rows, k = out.shape
+    index = dev.index
+    with _OnDevice(index):
+        status = lib.feather_mxfp4_dequantize(data.data_ptr(), scales.data_ptr(), rows, k, _SRC_CODE[out.dtype], out.data_ptr(), _raw_stream(index))
+    if status != FEATHER_OK:
+        _check(status, "feather_mxfp4_dequantize")
+    return out
+
+
+def mxfp4_mm_into(a, a_scales, b, b_scales, bias, c):
+    """c[:, :N] = round(a @ b^T + bias) with MXFP4 a [M, K/2] and b [N, K/2]; c may be a column slice of a wider row-major buffer."""
+    lib = load_library()
+    dev = _require_cuda(a, a_scales, b, b_scales, bias, c)
+    index = dev.index
+    st = status_word_for(dev)
+    with _OnDevice(index):
+        status = lib.feather_mxfp4_mm(
+            a.data_ptr(), a_scales.data_ptr(), b.data_ptr(), b_scales.data_ptr(), _addr(bias), c.data_ptr(), a.shape[0], b.shape[0], a.shape[1] * 2, c.stride(0),
+            _OUT_CODE[c.dtype], st.data_ptr(), _raw_stream(index),
+        )
+    if status != FEATHER_OK:
+        _check(status, "feather_mxfp4_mm")
+    return c
+
+
+def gated_norm(args, dev):
+    """Enqueues `feather_gated_norm` with a filled `NormArgs` on the current stream of `dev`."""
+    lib = load_library()
+    index = dev.index
+    with _OnDevice(index):
+        status = lib.feather_gated_norm(ctypes.byref(args), _raw_stream(index))
+    if status != FEATHER_OK:
+        _check(status, "feather_gated_norm")

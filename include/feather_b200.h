@@ -253,6 +253,76 @@ FEATHER_API int feather_dequantize(const uint8_t* src_prepacked, const float* sc
 FEATHER_API int feather_bf16_to_fp16(const uint16_t* src, uint16_t* dst, int64_t n, feather_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * MXFP4: the OCP microscaling format with 4-bit elements.  No counterpart in the reference.
+ *
+ * A row of K elements (K % 32 == 0) is cut into blocks of 32.  A block has one E8M0 scale byte `code` (the factor 2^(code - 127);
+ * 255 stands for NaN) and 32 E2M1 elements (0, .5, 1, 1.5, 2, 3, 4, 6 with a sign).  Storage:
+ *   data    [rows, K/2] bytes; byte j of a row holds element 2j in its low and 2j + 1 in its high nibble
+ *   scales  feather_mxfp4_scale_bytes(rows, K) bytes in tiles of 128 rows x 4 blocks: block kb of row r is byte
+ *           ((r/128) * ceil(K/128) + kb/4) * 512 + (r%32)*16 + (r/32%4)*4 + kb%4
+ *           A row's bytes past its last block are zero; bytes of rows past the last one are not written and may hold anything.
+ * ------------------------------------------------------------------------------------------- */
+
+/* Bytes of the tiled scales of a [rows, K] matrix.  No counterpart in the reference. */
+FEATHER_API size_t feather_mxfp4_scale_bytes(int64_t rows, int64_t K);
+
+/* src [rows, K] (FEATHER_SRC_* dtype, row pitch ld elements) -> MXFP4.  A block's scale is 2^(floor(log2 max|x|) - 2), at least
+ * 2^-127; elements are rounded to nearest even and saturate at 6.  A block that holds a NaN or an infinity gets the scale code 255
+ * and zero elements.  data and scales are 16-byte aligned.  No counterpart in the reference. */
+FEATHER_API int feather_mxfp4_quantize(const void* src, int src_dtype, int64_t rows, int64_t K, int64_t ld, uint8_t* data, uint8_t* scales,
+                           feather_stream_t stream);
+
+/* The values MXFP4 rows stand for, rounded to dst_dtype (FEATHER_SRC_* codes), dst [rows, K] row-major; everything 16-byte aligned.
+ * No counterpart in the reference. */
+FEATHER_API int feather_mxfp4_dequantize(const uint8_t* data, const uint8_t* scales, int64_t rows, int64_t K, int dst_dtype, void* dst,
+                             feather_stream_t stream);
+
+/* c[m, n] = round(sum_k a[m, k] * b[n, k] + bias[n]) with a [M, K] and b [N, K] in MXFP4, fp32 accumulation and one rounding to
+ * output_dtype (FEATHER_OUT_*).
+ *   a, b         data and scales as above, all 16-byte aligned
+ *   bias         output dtype [N] or NULL
+ *   c            output dtype [M, ldc], ldc >= N; only columns [0, N) of each row are written
+ *   status_dev   int32 device word or NULL; left untouched on success
+ * Needs no workspace and gives the same bits on every run.  No counterpart in the reference. */
+FEATHER_API int feather_mxfp4_mm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* b, const uint8_t* b_scales, const void* bias, void* c,
+                     int64_t M, int64_t N, int64_t K, int64_t ldc, int output_dtype, int* status_dev, feather_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Norms around a block, its gate and its residual.  No counterpart in the reference.
+ *
+ *   z = y, or norm(y) * post_weight with post_norm
+ *   r = x + residual_scale * gate * z
+ *   h = (norm(r) * weight + bias) * (1 + scale) + shift
+ *   norm(v) = v / sqrt(mean(v^2) + eps)  or  (v - mean(v)) / sqrt(mean((v - mean(v))^2) + eps), statistics in fp32
+ *
+ * x, y, r, h are [rows, cols] with row pitches ldx, ldy, ldr, ldh (elements); y, r, h and every vector may be NULL: without y the
+ * norm is that of x, without h only r is computed.  weight, bias, post_weight are [cols].  gate, scale and shift are matrices whose
+ * row i / gate_rows (scale_rows, shift_rows) belongs to row i of x, with row pitch gate_ld (scale_ld, shift_ld).
+ * With h_scales, h is MXFP4 data (ldh is ignored): the bits of feather_mxfp4_quantize over the h of type h_dtype.  That needs
+ * cols % 32 == 0 and 16-byte aligned rows everywhere.  cols is at most 16384.  r and h must not overlap an input.
+ * ------------------------------------------------------------------------------------------- */
+enum { FEATHER_NORM_RMS = 0, FEATHER_NORM_LAYER = 1 };
+typedef struct feather_norm_args {
+    const void *x, *y;
+    void *r, *h;
+    uint8_t* h_scales;
+    const void *weight, *bias, *post_weight, *gate, *scale, *shift;
+    int64_t rows, cols;
+    int64_t ldx, ldy, ldr, ldh;
+    int64_t gate_ld, scale_ld, shift_ld;
+    int64_t gate_rows, scale_rows, shift_rows;
+    float residual_scale, eps;
+    int kind;       /* FEATHER_NORM_* */
+    int post_norm;  /* 1: y goes through the norm (and post_weight) before the gate */
+    int x_dtype;    /* of x and r; FEATHER_SRC_* codes here and below */
+    int y_dtype, h_dtype;
+    int weight_dtype, bias_dtype, post_weight_dtype, gate_dtype, scale_dtype, shift_dtype;
+} feather_norm_args;
+
+/* The fused norm above; args_host is a host structure, read before the call returns.  No counterpart in the reference. */
+FEATHER_API int feather_gated_norm(const feather_norm_args* args_host, feather_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Library state
  * ------------------------------------------------------------------------------------------- */
 FEATHER_API const char* feather_last_error_string(void);
