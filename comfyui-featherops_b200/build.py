@@ -1,6 +1,7 @@
-"""Builds libfeather_b200.so (the C-ABI library declared in include/feather_b200.h) in-tree with nvcc for sm_100a.
+"""Builds libfeather_b200.so (the C-ABI library declared in include/feather_b200.h) in-tree with nvcc for sm_100a, and
+_feather_binding.so (the torch binding of the MXFP4 operators and the fused norm, csrc/binding.cpp) with the C++ compiler.
 
-Usage: ``python build.py`` from any directory, or ``build_library()`` from Python.  nvcc cross-compiles, so no GPU is
+Usage: ``python build.py`` from any directory, or ``build_library()`` and ``build_binding()`` from Python.  nvcc cross-compiles, so no GPU is
 needed to build.  The library links the CUDA runtime statically and resolves the one driver symbol it needs
 (cuTensorMapEncodeTiled) at run time, so it also loads on a machine without a driver (every call then reports an error).
 """
@@ -78,6 +79,37 @@ def build_library(force=False, verbose=False):
     return LIB_PATH
 
 
+BINDING_SRC = os.path.join(CSRC_DIR, "binding.cpp")
+BINDING_PATH = os.path.join(PKG_DIR, "_feather_binding.so")
+
+
+def build_binding(force=False):
+    """Compile csrc/binding.cpp against the installed torch into _feather_binding.so.  Returns its path.  The module takes the
+    entry points of libfeather_b200.so as addresses when it is loaded, so the two are built independently."""
+    import sysconfig
+
+    import torch
+
+    deps = [BINDING_SRC, os.path.join(PKG_DIR, "..", "include", "feather_b200.h"), torch.__file__]
+    if not force and os.path.exists(BINDING_PATH) and all(os.path.getmtime(d) <= os.path.getmtime(BINDING_PATH) for d in deps):
+        return BINDING_PATH
+    cxx = shutil.which("c++") or shutil.which("g++")
+    if cxx is None:
+        raise RuntimeError("no C++ compiler found: _feather_binding.so cannot be built")
+    torch_dir = os.path.dirname(torch.__file__)
+    include = os.path.join(torch_dir, "include")
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    tmp = BINDING_PATH + ".tmp"
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", include, "-I", os.path.join(include, "torch", "csrc", "api", "include"), "-I", sysconfig.get_paths()["include"], "-I", os.path.join(cuda, "include"),
+           BINDING_SRC, "-L", os.path.join(torch_dir, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python", "-o", tmp]
+    res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"torch binding failed to build:\n{res.stdout}")
+    os.replace(tmp, BINDING_PATH)
+    return BINDING_PATH
+
+
 CBENCH_SRC = os.path.join(PKG_DIR, "cbench", "bench_scaled_mm.c")
 CBENCH_BIN = os.path.join(PKG_DIR, "cbench", "bench_scaled_mm")
 
@@ -101,5 +133,6 @@ def build_cbench(cc=None):
 if __name__ == "__main__":
     path = build_library(force="--force" in sys.argv, verbose="-v" in sys.argv)
     print(path)
+    print(build_binding(force="--force" in sys.argv))
     if "--cbench" in sys.argv:
         print(build_cbench())

@@ -9,6 +9,8 @@ loads the HIP extension.
 """
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import threading
 
@@ -16,6 +18,7 @@ import torch
 
 _PKG_DIR = os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 LIB_PATH = os.path.join(_PKG_DIR, "libfeather_b200.so")
+BINDING_PATH = os.path.join(_PKG_DIR, "_feather_binding.so")
 
 FEATHER_OK = 0
 FEATHER_ERR_DEVICE_TIMEOUT = 5
@@ -635,30 +638,41 @@ def bf16_to_fp16(x):
 
 
 # ------------------------------------------------------------------------------------------------
-# MXFP4 and the fused norm
+# MXFP4 and the fused norm.  Their operators (kernel/mxfp4.py, kernel/norm.py) take a few microseconds on the GPU, so checks,
+# allocation and launch are one call into a C++ module (csrc/binding.cpp) that holds the C entry points' addresses.
 # ------------------------------------------------------------------------------------------------
-def mxfp4_quantize_into(x, data, scales):
-    """x [R, K] fp32 / bf16 / fp16 with unit column stride -> data [R, K/2], scales [ceil(R/128), ceil(K/128), 512] (uint8, contiguous)."""
-    lib = load_library()
-    dev = _require_cuda(x, data, scales)
-    rows, k = x.shape
-    index = dev.index
-    with _OnDevice(index):
-        status = lib.feather_mxfp4_quantize(x.data_ptr(), _SRC_CODE[x.dtype], rows, k, x.stride(0), data.data_ptr(), scales.data_ptr(), _raw_stream(index))
-    if status != FEATHER_OK:
-        _check(status, "feather_mxfp4_quantize")
+_binding = None
 
 
-def mxfp4_dequantize_into(data, scales, out):
+def _status_address(index):
+    return status_word_for(torch.device("cuda", index)).data_ptr()
+
+
+def _load_binding():
+    global _binding
     lib = load_library()
-    dev = _require_cuda(data, scales, out)
-    rows, k = out.shape
-    index = dev.index
-    with _OnDevice(index):
-        status = lib.feather_mxfp4_dequantize(data.data_ptr(), scales.data_ptr(), rows, k, _SRC_CODE[out.dtype], out.data_ptr(), _raw_stream(index))
-    if status != FEATHER_OK:
-        _check(status, "feather_mxfp4_dequantize")
-    return out
+    with _lib_lock:
+        if _binding is not None:
+            return _binding
+        if not os.path.exists(BINDING_PATH):
+            raise FeatherNativeError(
+                f"{BINDING_PATH} is missing. Build it with `python {os.path.join(_PKG_DIR, 'build.py')}` "
+                "(needs a C++ compiler; there is no fallback implementation)."
+            )
+        loader = importlib.machinery.ExtensionFileLoader("_feather_binding", BINDING_PATH)
+        mod = importlib.util.module_from_spec(importlib.util.spec_from_file_location("_feather_binding", BINDING_PATH, loader=loader))
+        loader.exec_module(mod)
+        if mod.torch_version != torch.__version__.split("+")[0]:
+            raise FeatherNativeError(f"{BINDING_PATH} was built for torch {mod.torch_version}, this is {torch.__version__}: run build.py again")
+        entries = (lib.feather_mxfp4_quantize, lib.feather_mxfp4_dequantize, lib.feather_mxfp4_mm, lib.feather_gated_norm, lib.feather_last_error_string)
+        mod.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in entries), FeatherNativeError, _status_address)
+        _binding = mod
+    return _binding
+
+
+def binding():
+    """The C++ module of the MXFP4 operators and the fused norm, loaded once.  Raises if it has not been built."""
+    return _binding if _binding is not None else _load_binding()
 
 
 def mxfp4_mm_into(a, a_scales, b, b_scales, bias, c):
@@ -675,13 +689,3 @@ def mxfp4_mm_into(a, a_scales, b, b_scales, bias, c):
     if status != FEATHER_OK:
         _check(status, "feather_mxfp4_mm")
     return c
-
-
-def gated_norm(args, dev):
-    """Enqueues `feather_gated_norm` with a filled `NormArgs` on the current stream of `dev`."""
-    lib = load_library()
-    index = dev.index
-    with _OnDevice(index):
-        status = lib.feather_gated_norm(ctypes.byref(args), _raw_stream(index))
-    if status != FEATHER_OK:
-        _check(status, "feather_gated_norm")
