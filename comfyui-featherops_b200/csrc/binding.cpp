@@ -358,6 +358,7 @@ PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.gate_rows = check_modulation(gate, "gate", x);
     a.scale_rows = check_modulation(scale, "scale", x);
     a.shift_rows = check_modulation(shift, "shift", x);
+    a.status_dev = status_word(device.index());
 
     at::Tensor r, h, h_scales;
     int status = FEATHER_OK;

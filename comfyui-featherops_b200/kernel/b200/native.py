@@ -82,6 +82,7 @@ class NormArgs(ctypes.Structure):
         + [(name, ctypes.c_float) for name in ("residual_scale", "eps")]
         + [(name, ctypes.c_int) for name in ("kind", "post_norm", "x_dtype", "y_dtype", "h_dtype", "weight_dtype", "bias_dtype", "post_weight_dtype",
                                              "gate_dtype", "scale_dtype", "shift_dtype")]
+        + [("status_dev", ctypes.c_void_p)]
     )
 
 

@@ -317,6 +317,7 @@ typedef struct feather_norm_args {
     int x_dtype;    /* of x and r; FEATHER_SRC_* codes here and below */
     int y_dtype, h_dtype;
     int weight_dtype, bias_dtype, post_weight_dtype, gate_dtype, scale_dtype, shift_dtype;
+    int* status_dev; /* int32 device word or NULL; left untouched on success */
 } feather_norm_args;
 
 /* The fused norm above; args_host is a host structure, read before the call returns.  No counterpart in the reference. */

@@ -60,6 +60,38 @@ def test_many_rows_take_the_wide_threads(norm, cuda_dev):
             _check(norm, x, y, gate=_t((cols,), 3, cuda_dev), post_norm=True, scale=_t((cols,), 4, cuda_dev, spread=0.2), shift=_t((cols,), 5, cuda_dev), kind=kind)
 
 
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("cols", [8, 40, 64, 256, 264, 320, 512, 520, 1000, 1024, 1032, 2048, 2560, 4096, 5120, 5128, 6144, 8192, 8200, 13824, 16384])
+def test_thousands_of_rows(norm, mx, cuda_dev, cols, kind):
+    """The form for many rows: samples that end inside a wave of rows, whole and partial vectors, all three coefficients or none, h alone
+    and r alone, and the MXFP4 result."""
+    batch, length = 3, 1601 if cols <= 2560 else 901
+    x, y = _t((batch, length, cols), 1, cuda_dev, BF16), _t((batch, length, cols), 2, cuda_dev, BF16)
+    kw = dict(gate=_t((batch, 1, cols), 3, cuda_dev), scale=_t((batch, 1, cols), 4, cuda_dev, spread=0.2), shift=_t((batch, 1, cols), 5, cuda_dev), kind=kind)
+    r, h = _check(norm, x, y, post_norm=True, post_weight=_t((cols,), 6, cuda_dev, BF16, 0.2, 1.0), **kw)
+    _check(norm, x, y, kind=kind)
+    _check(norm, x, None, kind=kind, weight=_t((cols,), 7, cuda_dev, FP16, 0.2, 1.0), bias=_t((cols,), 8, cuda_dev))
+    alone, none = norm.gated_residual_norm(x, y, gate=kw["gate"], kind=kind, want_norm=False)
+    both, _ = norm.gated_residual_norm(x, y, gate=kw["gate"], kind=kind)
+    assert none is None and torch.equal(alone, both)
+    if cols % 32 == 0:
+        _, h = norm.gated_residual_norm(x, y, **kw)
+        _, (data, scales) = norm.gated_residual_norm(x, y, packed=True, **kw)
+        ref_data, ref_scales = mx.quantize_mxfp4(h.view(-1, cols))
+        assert torch.equal(data, ref_data)
+        assert torch.equal(mx.unprepack_mxfp4_scales(scales, batch * length, cols), mx.unprepack_mxfp4_scales(ref_scales, batch * length, cols))
+
+
+@pytest.mark.parametrize("x_dtype,y_dtype", [(FP32, FP32), (FP32, FP16), (FP16, BF16), (BF16, FP32)])
+def test_thousands_of_rows_of_other_types(norm, cuda_dev, x_dtype, y_dtype):
+    for cols in (200, 1024, 5120, 12288):
+        x, y = _t((5, 701, cols), 1, cuda_dev, x_dtype, about=3.0), _t((5, 701, cols), 2, cuda_dev, y_dtype)
+        _check(norm, x, y, gate=_t((5, 1, cols), 3, cuda_dev, y_dtype), post_norm=True, shift=_t((cols,), 4, cuda_dev), kind="layer")
+        wide = torch.zeros((3505, cols + 16), dtype=x_dtype, device=cuda_dev)
+        wide[:, 8:-8] = x.view(-1, cols)
+        _check(norm, wide[:, 8:-8], y.view(-1, cols), residual_scale=0.25)
+
+
 @pytest.mark.parametrize("x_dtype", [BF16, FP16, FP32])
 @pytest.mark.parametrize("y_dtype", [BF16, FP16, FP32])
 def test_types(norm, cuda_dev, x_dtype, y_dtype):
