@@ -70,26 +70,33 @@ __device__ __forceinline__ void mx_unpack8(uint32_t w, float (&v)[8]) {
     }
 }
 
+// Scale code of a block whose largest |x| has these fp32 bits.  As unsigned integers the bits of |x| order like the values, with every
+// NaN above infinity.
+__device__ __forceinline__ uint32_t mx_code(uint32_t top) {
+    const uint32_t exponent = top >> 23;
+    return exponent == 255u ? 255u : exponent > 2u ? exponent - 2u : 0u;
+}
+
+// Eight values -> codes under a block's scale.
+__device__ __forceinline__ uint32_t mx_scaled_pack8(const float (&x)[8], uint32_t code) {
+    if (code == 255u) return 0u;
+    const float inverse = __uint_as_float((254u - code) << 23);      // 2^(127 - code): a normal number, the product is exact
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = x[i] * inverse;
+    return mx_pack8(v);
+}
+
 // One block of 32 is held by four neighbouring lanes, eight elements each (lane % 4 = position); every lane of the warp calls
 // this, a lane without elements with zeros.  Returns the lane's eight codes; `code` is the block's scale.
-// As unsigned integers the bit patterns of |x| order like the values, with every NaN above infinity.
 __device__ __forceinline__ uint32_t mx_quantize8(const float (&x)[8], uint32_t& code) {
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const uint32_t exponent = top >> 23;
-    if (exponent == 255u) {
-        code = 255u;
-        return 0u;
-    }
-    code = exponent > 2u ? exponent - 2u : 0u;
-    const float inverse = __uint_as_float((254u - code) << 23);      // 2^(127 - code): a normal number, the product is exact
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = x[i] * inverse;
-    return mx_pack8(v);
+    code = mx_code(top);
+    return mx_scaled_pack8(x, code);
 }
 
 // The scale bytes of the four blocks that 16 neighbouring lanes hold, as one word (the same on all 16).  Lanes beyond the row's
