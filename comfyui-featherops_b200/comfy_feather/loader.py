@@ -1,5 +1,6 @@
 """ComfyUI node `FeatherUNetLoader` (reference: comfy_feather/loader.py:9-77): loads a diffusion model with
-`custom_operations = feather_ops(out_dtype, excluded_names)` so every eligible Linear becomes a Feather linear.
+`custom_operations = feather_ops(out_dtype, excluded_names, weight_format)` so every eligible Linear becomes a Feather linear
+(the optional weight_format, "mxfp4" instead of the reference's "fp8e5m2", is this repository's own).
 The reference's loader also installs a sampling-time model pin (comfy_feather/sampling.py:64-83), ComfyUI memory-management
 bookkeeping that is not part of the linear path and is not rebuilt here."""
 
@@ -30,15 +31,17 @@ class FeatherUNetLoader:
             "required": {
                 "unet_name": (folder_paths.get_filename_list("diffusion_models"),),
                 "model_type": (list(MODEL_TYPES),),
-            }
+            },
+            "optional": {"weight_format": (["fp8e5m2", "mxfp4"],)},
         }
 
     RETURN_TYPES = ("MODEL",)
     FUNCTION = "load_unet"
     CATEGORY = "loaders"
 
-    def load_unet(self, unet_name, model_type):
+    def load_unet(self, unet_name, model_type, weight_format="fp8e5m2"):
         unet_path = folder_paths.get_full_path_or_raise("diffusion_models", unet_name)
         excluded, out_dtype = MODEL_TYPES.get(model_type, MODEL_TYPES["default"])
-        model = load_diffusion_model(unet_path, model_options={"custom_operations": feather_ops(out_dtype=out_dtype, excluded_names=list(excluded))})
+        operations = feather_ops(out_dtype=out_dtype, excluded_names=list(excluded), weight_format=weight_format)
+        model = load_diffusion_model(unet_path, model_options={"custom_operations": operations})
         return (model,)

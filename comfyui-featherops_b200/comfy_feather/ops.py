@@ -1,4 +1,4 @@
-"""`feather_ops(out_dtype, excluded_names)` -> a ComfyUI custom-operations class whose `Linear` keeps its weight as
+"""`feather_ops(out_dtype, excluded_names, weight_format)` -> a ComfyUI custom-operations class whose `Linear` keeps its weight as
 prepacked fp8e5m2 and runs the sm_100a mixed-precision GEMM.
 
 Same surface and behaviour as the reference's comfy_feather/ops.py:17-148 (state-dict loading with `weight_scale` /
@@ -7,6 +7,9 @@ with two differences in `forward`: the reference pads the token count up to a mu
 (ops.py:126-139) because its kernel needs tile-divisible M; the B200 kernel handles ragged M itself, so no padded copy
 is made and the rows beyond M never exist.  And the cast of the result back to the model's dtype (ops.py:103) is folded
 into the GEMM's epilogue.
+
+`weight_format="mxfp4"` (not in the reference) keeps the weight as MXFP4 instead: half the bytes, and the activations are quantised
+to MXFP4 on the way in, so that the product runs on the 4-bit tensor-core path.
 """
 
 import torch
@@ -16,7 +19,9 @@ from torch import nn
 
 from ..kernel.convert import bf16_to_fp16
 from ..kernel.hip.hip_kernel import scaled_mm_b200, scaled_mm_lora
+from ..kernel.mxfp4 import linear_mxfp4
 from .lora import apply_lora_patches, fused_lora_operands
+from .mxfp4 import get_mxfp4_plain_tensors, is_mxfp4_weight, make_mxfp4_weight, quantize_mxfp4_weight
 from .quant import get_feather_plain_tensors, is_feather_quantized_weight, make_feather_quantized_weight, quantize_feather_weight
 
 
@@ -132,14 +137,71 @@ class _FeatherLinear:
         return y, fused is not None
 
 
-def feather_ops(out_dtype=torch.bfloat16, excluded_names=()):
-    """The operations class ComfyUI instantiates the model with: `manual_cast` whose `Linear` is the quantised linear."""
-    names, dtype = tuple(excluded_names), out_dtype
+class _FeatherMXFP4Linear(_FeatherLinear):
+    """The same Linear with an MXFP4 weight.  Un-merged LoRA patches are added after the product."""
+
+    def _keeps_plain_weight(self, prefix, weight):
+        return super()._keeps_plain_weight(prefix, weight) or self.in_features % 32 != 0
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        weight, bias, weight_scale, legacy_scale = (state_dict.pop(prefix + key, None) for key in _STATE_KEYS)
+        if weight is None:
+            missing_keys.append(prefix + "weight")
+        else:
+            self.is_quantized = not self._keeps_plain_weight(prefix, weight)
+            scale = weight_scale if weight_scale is not None else legacy_scale
+            if self.is_quantized:
+                weight = make_mxfp4_weight(weight, scale, self.out_dtype)
+            elif weight.dtype == torch.uint8:                      # MXFP4 in the checkpoint, excluded here
+                weight = make_mxfp4_weight(weight, scale, self.out_dtype).dequantize()
+            elif self.in_features % 32 != 0:
+                print(f"Warning: Not MXFP4 {prefix}weight {tuple(weight.shape)}")
+            self.weight = _frozen(weight)
+        self.bias = None if bias is None else _frozen(bias.to(self.out_dtype))
+
+    def convert_weight(self, weight, inplace=False, **kwargs):
+        if self.is_quantized and not is_mxfp4_weight(weight):
+            raise TypeError(f"Expected an MXFP4 weight, got {type(weight).__name__}")
+        return weight.dequantize() if self.is_quantized else weight
+
+    def set_weight(self, weight, inplace_update=False, seed=None, return_weight=False, **kwargs):
+        merged = quantize_mxfp4_weight(weight) if self.is_quantized else weight.to(self.weight.dtype)
+        if return_weight:
+            return merged
+        assert inplace_update is False
+        self.weight = _frozen(merged)
+
+    def _forward_quantized(self, x, lora_functions=()):
+        dtype_orig = x.dtype
+        if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            x = x.to(self.out_dtype)
+        saved_weight_function = self.weight_function
+        self.weight_function = []                                  # cast_bias_weight must not apply low-VRAM LoRA patches to the packed weight
+        try:
+            bias_dtype = self.bias.dtype if self.bias is not None else None
+            weight, bias, offload_stream = cast_bias_weight(self, x, dtype=self.weight.dtype, bias_dtype=bias_dtype, offloadable=True)
+            data, scales = get_mxfp4_plain_tensors(weight)
+            y = linear_mxfp4(x, data, scales, bias, self.out_dtype)
+            uncast_bias_weight(self, weight, bias, offload_stream)
+        finally:
+            self.weight_function = saved_weight_function
+        return y if y.dtype == dtype_orig else y.to(dtype_orig), False
+
+
+_LINEARS = {"fp8e5m2": _FeatherLinear, "mxfp4": _FeatherMXFP4Linear}
+
+
+def feather_ops(out_dtype=torch.bfloat16, excluded_names=(), weight_format="fp8e5m2"):
+    """The operations class ComfyUI instantiates the model with: `manual_cast` whose `Linear` is the quantised linear, with the
+    weight as prepacked fp8e5m2 (the reference's format) or as MXFP4."""
+    if weight_format not in _LINEARS:
+        raise ValueError(f"unknown weight_format {weight_format!r} (expected one of {', '.join(_LINEARS)})")
+    names, dtype, base = tuple(excluded_names), out_dtype, _LINEARS[weight_format]
 
     class FeatherOps(manual_cast):
         _excluded_names, _out_dtype = names, dtype
 
-        class Linear(_FeatherLinear, manual_cast.Linear):
+        class Linear(base, manual_cast.Linear):
             excluded_names = names
             out_dtype = dtype
 

@@ -29,6 +29,11 @@ Multi-GPU modes (one process per GPU, the same seeded weights generated on every
                    is bitwise the 1-GPU linear on the same input; attention runs on another query partition, so the forward
                    is compared within tolerance.
 
+`weight_format="mxfp4"` (one rank) is the same block with MXFP4 linears and fused norms: each norm, the gated residual in front of it and
+the quantisation of its result are one pass (`gated_residual_norm`) whose output the next linear multiplies as it is.  Its forward also
+takes a modulation, the (shift, scale, gate) of both halves of every block:
+    h = rmsnorm(x) (1 + scale1) + shift1;  x = x + gate1 * Wo sdpa(...);  h = rmsnorm(x) (1 + scale2) + shift2;  x = x + gate2 * Wdown gelu(Wup h)
+
 `linear_factory` exists so tests can run the same forward on CPU ranks with the CPU oracle standing in for the CUDA GEMM;
 the default factory is the CUDA path and raises without a GPU.
 """
@@ -38,6 +43,8 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 
+from ..mxfp4 import MXFP4Linear
+from ..norm import gated_residual_norm
 from . import native
 from .sharded import ColumnShardedLinear, ReplicatedLinear, RowGather, RowShardedLinear
 
@@ -104,7 +111,11 @@ def rmsnorm(x, gain, eps):
 
 class FeatherDiT:
     def __init__(self, cfg, rank=0, world=1, device=None, mode="all_gather", exchange="peer_store", seed=0, linear_factory=None,
-                 init_device=None, group=None):
+                 init_device=None, group=None, weight_format="fp8e5m2"):
+        if weight_format not in ("fp8e5m2", "mxfp4"):
+            raise ValueError(f"unknown weight_format {weight_format!r}")
+        if weight_format == "mxfp4" and (world != 1 or linear_factory is not None):
+            raise ValueError("the MXFP4 forward runs on one rank, without a linear_factory")
         if mode not in ("all_gather", "pairs", "tokens"):
             raise ValueError(f"unknown mode {mode!r}")
         if cfg.hidden != cfg.heads * cfg.head_dim:
@@ -119,6 +130,7 @@ class FeatherDiT:
         gen = torch.Generator(device=init_device).manual_seed(seed)
         h, f = cfg.hidden, cfg.ffn
         pairs = mode == "pairs"
+        self.weight_format = weight_format
         self._gathers = {}
 
         def weight(n, k):
@@ -133,7 +145,10 @@ class FeatherDiT:
             b["norm1"] = (1.0 + vector(h, 0.1)).to(self.device, torch.bfloat16)
             b["norm2"] = (1.0 + vector(h, 0.1)).to(self.device, torch.bfloat16)
             q_gain, k_gain = (1.0 + vector(h, 0.1)), (1.0 + vector(h, 0.1))
-            if mode == "tokens":
+            if weight_format == "mxfp4":
+                for name, n, k in (("q", h, h), ("k", h, h), ("v", h, h), ("o", h, h), ("up", f, h), ("down", h, f)):
+                    b[name] = MXFP4Linear(weight(n, k), vector(n, 0.1).to(torch.bfloat16), self.device)
+            elif mode == "tokens":
                 # the same draws in the same order as the other modes, every weight whole
                 for name, n, k in (("q", h, h), ("k", h, h), ("v", h, h), ("o", h, h), ("up", f, h), ("down", h, f)):
                     b[name] = self.factory.full(weight(n, k), vector(n, 0.1))
@@ -204,9 +219,42 @@ class FeatherDiT:
             xl = call(blk["down"], "down", i, u16, residual=xl)
         return self.factory.gather_rows(xl)
 
-    def forward(self, x, hook=None):
+    def _forward_mxfp4(self, x, hook, modulation):
+        """x [T, hidden] or [B, T, hidden] bf16; modulation [blocks, 6, hidden] or [blocks, 6, B, 1, hidden]: shift, scale and gate of
+        the attention half, then of the feed-forward half, of every block."""
+        cfg, bf16 = self.cfg, torch.bfloat16
+        shape = x.shape
+
+        def call(lin, name, i, a):
+            y = lin(a, bf16)
+            if hook is not None:
+                hook(name, i, a, y)
+            return y
+
+        def norm(x, y, gain, gate, shift, scale):
+            return gated_residual_norm(x, y, gate=gate, weight=gain, shift=shift, scale=scale, eps=cfg.eps, out_dtype=bf16, packed=True)
+
+        nothing = (None,) * 6
+        y = gate = None
+        for i, blk in enumerate(self.blocks):
+            shift1, scale1, gate1, shift2, scale2, gate2 = nothing if modulation is None else modulation[i]
+            x, h = norm(x, y, blk["norm1"], gate, shift1, scale1)
+            q, k, v = (call(blk[name], name, i, h).view(-1, *shape[-2:]) for name in "qkv")
+            attn = torch.cat([self._attention(q[b], k[b], v[b], blk) for b in range(q.shape[0])])
+            y = call(blk["o"], "o", i, attn).view(shape)
+            x, h = norm(x, y, blk["norm2"], gate1, shift2, scale2)
+            y = call(blk["down"], "down", i, F.gelu(call(blk["up"], "up", i, h), approximate="tanh")).view(shape)
+            gate = gate2
+        return x if y is None else gated_residual_norm(x, y, gate=gate, want_norm=False)[0]
+
+    def forward(self, x, hook=None, modulation=None):
         """x [T, hidden] bf16 (the same on every rank) -> [T, hidden] bf16 (the same on every rank).
-        `hook(name, block, input_fp16, output)` sees every linear's input and output (tests use it)."""
+        `hook(name, block, input_fp16, output)` sees every linear's input and output (tests use it); an MXFP4 linear's input is
+        the 16-bit tensor or the (data, scales) pair it was given.  modulation: of the MXFP4 forward only."""
+        if self.weight_format == "mxfp4":
+            return self._forward_mxfp4(x, hook, modulation)
+        if modulation is not None:
+            raise ValueError("a modulation needs weight_format='mxfp4'")
         if self.mode == "tokens":
             return self._forward_tokens(x, hook)
         cfg, bf16 = self.cfg, torch.bfloat16

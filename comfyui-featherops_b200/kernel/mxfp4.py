@@ -118,3 +118,19 @@ def linear_mxfp4(x: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, bias:
     if torch.compiler.is_compiling():
         return _linear_op(x, b, b_scales, bias, out_dtype)
     return native.binding().linear(x, b, b_scales, bias, out_dtype)
+
+
+class MXFP4Linear:
+    """y = round(x @ W^T + bias) with the weight held as MXFP4; x is a tensor, quantised on the way in, or the pair (data, scales) that
+    `quantize_mxfp4` and `gated_residual_norm(..., packed=True)` give."""
+
+    def __init__(self, weight, bias=None, device=None):
+        """weight [N, K] fp32 / bf16 / fp16, bias [N] or None; both are taken to `device` (default: the weight's)."""
+        device = weight.device if device is None else device
+        self.data, self.scales = quantize_mxfp4(weight.to(device))
+        self.bias = None if bias is None else bias.to(device).contiguous()
+
+    def __call__(self, x, out_dtype=torch.bfloat16):
+        if isinstance(x, tuple):
+            return scaled_mm_mxfp4(*x, self.data, self.scales, self.bias, out_dtype)
+        return linear_mxfp4(x, self.data, self.scales, self.bias, out_dtype)

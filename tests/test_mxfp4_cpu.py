@@ -191,3 +191,34 @@ def test_c_entries_check_their_arguments(native):
     ):
         says(lib.feather_gated_norm(ctypes.byref(args(**kw)), null), code, text)
     says(lib.feather_gated_norm(None, null), 1, b"null")
+
+
+def test_operations_and_loader_take_a_weight_format(pkg):
+    ops_mod = importlib.import_module("feather_b200.comfy_feather.ops")
+    loader = importlib.import_module("feather_b200.comfy_feather.loader")
+    layout = importlib.import_module("feather_b200.comfy_feather.mxfp4")
+    import comfy.sd
+
+    with pytest.raises(ValueError, match="weight_format"):
+        ops_mod.feather_ops(weight_format="nvfp4")
+    assert loader.FeatherUNetLoader.INPUT_TYPES()["optional"]["weight_format"][0] == ["fp8e5m2", "mxfp4"]
+    loader.FeatherUNetLoader().load_unet("model_a.safetensors", "wan", "mxfp4")
+    ops = comfy.sd._last_call["model_options"]["custom_operations"]
+    assert issubclass(ops.Linear, ops_mod._FeatherMXFP4Linear) and ops._out_dtype == torch.float16
+    loader.FeatherUNetLoader().load_unet("model_a.safetensors", "wan")
+    assert not issubclass(comfy.sd._last_call["model_options"]["custom_operations"].Linear, ops_mod._FeatherMXFP4Linear)
+
+    # a packed checkpoint needs no GPU to load; its values come back as they were saved
+    lin = ops_mod.feather_ops(weight_format="mxfp4").Linear(96, 40, bias=False)
+    data = torch.randint(0, 256, (40, 48), generator=torch.Generator().manual_seed(1)).to(torch.uint8)
+    scale = torch.randint(100, 140, (40, 3), generator=torch.Generator().manual_seed(2)).to(torch.uint8)
+    lin._load_from_state_dict({"l.weight": data, "l.weight_scale": scale}, "l.", {}, True, [], [], [])
+    assert lin.is_quantized and tuple(lin.weight.shape) == (40, 96)
+    saved = layout.FeatherMXFP4Layout.state_dict_tensors(lin.weight._qdata, lin.weight._params)
+    assert torch.equal(saved[""], data) and torch.equal(saved["_scale"], scale)
+    with pytest.raises(ValueError, match="recalculate"):
+        layout.FeatherMXFP4Layout.quantize(torch.zeros((4, 32)), scale=torch.tensor(1.0))
+    with pytest.raises(ValueError, match="divisible by 32"):
+        layout.quantize_mxfp4_weight(torch.zeros((4, 48)))
+    with pytest.raises(TypeError, match="FeatherMXFP4Layout"):
+        layout.get_mxfp4_plain_tensors(torch.zeros(4))
