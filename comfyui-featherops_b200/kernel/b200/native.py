@@ -646,6 +646,10 @@ _binding = None
 
 
 def _status_address(index):
+    """Address of the device's status word; 0 (no status for this call) where it would have to be allocated inside a graph capture,
+    whose memory and zero fill belong to the graph."""
+    if ("cuda", index) not in _status_words and torch.cuda.is_current_stream_capturing():
+        return 0
     return status_word_for(torch.device("cuda", index)).data_ptr()
 
 

@@ -109,7 +109,9 @@ def _operand(mx, rows, k, seed, dev, spread=3):
 
 
 SHAPES = [(1, 1, 32), (1, 8, 64), (1, 128, 256), (2, 130, 96), (5, 257, 160), (16, 384, 512), (17, 129, 1056), (31, 640, 800), (33, 1000, 288), (64, 128, 2048), (65, 511, 320),
-          (128, 256, 1024), (129, 384, 544), (200, 1024, 384), (255, 777, 1312), (257, 256, 256), (520, 2811, 1056), (1000, 520, 640), (1, 5120, 13824), (7, 1100, 4096)]
+          (128, 256, 1024), (129, 384, 544), (200, 1024, 384), (255, 777, 1312), (257, 256, 256), (520, 2811, 1056), (1000, 520, 640), (1, 5120, 13824), (7, 1100, 4096),
+          (300, 1, 64), (70, 8, 32), (1000, 100, 96), (2100, 193, 160), (64, 3, 13824), (4099, 1537, 96),
+          (2048, 4608, 2048), (1999, 4601, 2016)]                           # enough tiles and stages for the 256-feature tile
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -244,3 +246,95 @@ def test_custom_ops_and_fakes(mx, cuda_dev):
         assert fd.shape == data.shape and fs.shape == scales.shape and fd.dtype == fs.dtype == torch.uint8
         fy = torch.ops.feather_ops_internal.scaled_mm_mxfp4(fd, fs, fd, fs, None, torch.float16)
         assert fy.shape == y.shape and fy.dtype == y.dtype
+
+
+def test_first_call_inside_a_capture(tmp_path):
+    """A process whose first calls of these operators are captured: the graph replays right, nothing kept from the capture (a status word)
+    outlives it, and eager calls follow."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    script = tmp_path / "first.py"
+    script.write_text("""
+import gc, importlib, sys
+sys.path.insert(0, %r)
+import torch, __graft_entry__
+__graft_entry__.load_package()
+mx = importlib.import_module("feather_b200.kernel.mxfp4")
+norm = importlib.import_module("feather_b200.kernel.norm").gated_residual_norm
+native = importlib.import_module("feather_b200.kernel.b200.native")
+w, x = torch.randn((640, 512), device="cuda"), torch.randn((2500, 512), device="cuda", dtype=torch.bfloat16)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    b = mx.quantize_mxfp4(w)
+    r, h = norm(x, x, gate=w[0], packed=True)
+    out = mx.scaled_mm_mxfp4(*h, *b), mx.linear_mxfp4(x[:5], *b), r
+g.replay()
+torch.cuda.synchronize()
+got = [o.clone() for o in out]
+del g, b, r, h, out
+gc.collect()
+torch.cuda.empty_cache()
+b = mx.quantize_mxfp4(w)
+r, h = norm(x, x, gate=w[0], packed=True)
+ref = mx.scaled_mm_mxfp4(*h, *b), mx.linear_mxfp4(x[:5], *b), r
+native.check_device_status()
+assert all(torch.equal(a, c) for a, c in zip(got, ref))
+print("captured first")
+""" % root)
+    res = subprocess.run([sys.executable, str(script)], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=120)
+    assert res.returncode == 0 and "captured first" in res.stdout, res.stdout[-2000:]
+
+
+def test_threads_on_streams_of_their_own(mx, cuda_dev):
+    """Several threads at once, each on its own stream: few tokens (clusters), many tokens (pairs) and the norm in between."""
+    import threading
+
+    norm = importlib.import_module("feather_b200.kernel.norm").gated_residual_norm
+    b, sb = mx.quantize_mxfp4(torch.randn((768, 640), generator=torch.Generator().manual_seed(1)).to(cuda_dev))
+    xs = [torch.randn((m, 640), generator=torch.Generator().manual_seed(m)).to(torch.bfloat16).to(cuda_dev) for m in (1, 40, 300, 2600)]
+
+    def step(x):
+        r, h = norm(x, x, post_norm=True, packed=True)
+        return r, mx.scaled_mm_mxfp4(*h, b, sb), mx.linear_mxfp4(x, b, sb)
+
+    ref = [step(x) for x in xs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = step(xs[i])
+            torch.cuda.current_stream().synchronize()
+            if not all(torch.equal(a, c) for a, c in zip(got, ref[i])):
+                wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(xs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_fakes_of_the_other_operators(mx, cuda_dev):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    importlib.import_module("feather_b200.kernel.norm")
+    ops = torch.ops.feather_ops_internal
+    x = torch.randn((2, 40, 128), device=cuda_dev, dtype=torch.bfloat16)
+    data, scales = mx.quantize_mxfp4(x[0])
+
+    def results(x, data, scales):
+        n = (x, x, None, 1.0, False, None, None, None, None, None, "rms", 1e-6)
+        return [ops.dequantize_mxfp4(data, scales, torch.float16), ops.linear_mxfp4(x, data, scales, None, None), *ops.gated_residual_norm(*n, torch.bfloat16, True, False),
+                *ops.gated_residual_norm(*n, torch.bfloat16, True, True), *ops.gated_residual_norm(*n, torch.bfloat16, False, False), *ops.gated_residual_norm(x, *[None] * 2, *n[3:], torch.float32, True, False)]
+
+    real = results(x, data, scales)
+    with FakeTensorMode():
+        fake = results(*(torch.empty(t.shape, dtype=t.dtype, device="cuda") for t in (x, data, scales)))
+    assert [(t.shape, t.dtype) for t in real] == [(t.shape, t.dtype) for t in fake]
