@@ -175,8 +175,10 @@ __host__ __device__ __forceinline__ int norm_present(const feather_norm_args& a)
 struct ModulationAt {
     long long gate, scale, shift;
 };
+__device__ __forceinline__ long long share_of(long long row, int64_t rows) { return static_cast<uint32_t>(row) / static_cast<uint32_t>(rows); }   // both fit (host)
 __device__ __forceinline__ ModulationAt modulation_at(const feather_norm_args& a, long long row) {
-    return {a.gate != nullptr ? row / a.gate_rows * a.gate_ld : 0, a.scale != nullptr ? row / a.scale_rows * a.scale_ld : 0, a.shift != nullptr ? row / a.shift_rows * a.shift_ld : 0};
+    return {a.gate != nullptr ? share_of(row, a.gate_rows) * a.gate_ld : 0, a.scale != nullptr ? share_of(row, a.scale_rows) * a.scale_ld : 0,
+            a.shift != nullptr ? share_of(row, a.shift_rows) * a.shift_ld : 0};
 }
 
 __device__ __forceinline__ void fold_g(const feather_norm_args& a, const RawAny& gate, const RawAny& post_weight, float (&u)[8]) {
@@ -226,9 +228,9 @@ __device__ __forceinline__ void finish_ab(const feather_norm_args& a, const RawA
 // First row after `row` that belongs to another row of gate, scale or shift.
 __device__ __forceinline__ long long next_change(const feather_norm_args& a, long long row) {
     long long change = a.rows;
-    if (a.gate != nullptr) change = min(change, (row / a.gate_rows + 1) * a.gate_rows);
-    if (a.scale != nullptr) change = min(change, (row / a.scale_rows + 1) * a.scale_rows);
-    if (a.shift != nullptr) change = min(change, (row / a.shift_rows + 1) * a.shift_rows);
+    if (a.gate != nullptr) change = min(change, (share_of(row, a.gate_rows) + 1) * a.gate_rows);
+    if (a.scale != nullptr) change = min(change, (share_of(row, a.scale_rows) + 1) * a.scale_rows);
+    if (a.shift != nullptr) change = min(change, (share_of(row, a.shift_rows) + 1) * a.shift_rows);
     return change;
 }
 
@@ -599,9 +601,10 @@ __global__ void __maxnreg__(norm_regs(NV)) gated_norm_groups_kernel(const __grid
     }
 }
 
-// Few rows, or a modulation for each row: a block takes one row, and gate, scale and shift are on their way together with x and y.
-template <int XT, int YT>
-__global__ void __launch_bounds__(1024) gated_norm_row_kernel(const __grid_constant__ NormParams p) {
+// Few rows, or a modulation for each row: a block takes one row.  DENSE: 48 registers instead of 64, with spills, so that two blocks of a
+// wide row fit an SM (4096 x 5120 bf16 with fp32 modulation of each row: 129 -> 101 us); one row alone takes 4.6 us that way, 4.1 us otherwise.
+template <int XT, int YT, bool DENSE>
+__global__ void __maxnreg__(DENSE ? 48 : 64) gated_norm_row_kernel(const __grid_constant__ NormParams p) {
     __shared__ __align__(16) float part[2][kNormMaxWarps];
     const feather_norm_args& a = p.a;
     clear_parts(part);
@@ -614,7 +617,7 @@ __global__ void __launch_bounds__(1024) gated_norm_row_kernel(const __grid_const
     const ModulationAt m = modulation_at(a, row);
     Raw8<XT> xr[1];
     Raw8<YT> yr[1];
-    RawAny gate, post_weight, scale, shift;
+    RawAny gate, post_weight;
     if (in) {
         if (a.y != nullptr) {
             yr[0] = load8<YT>(a.y, row * a.ldy + at);
@@ -622,8 +625,6 @@ __global__ void __launch_bounds__(1024) gated_norm_row_kernel(const __grid_const
             load_any(post_weight, a.post_weight, a.post_weight_dtype, at);
         }
         xr[0] = load8<XT>(a.x, row * a.ldx + at);
-        load_any(scale, a.scale, a.scale_dtype, m.scale + at);
-        load_any(shift, a.shift, a.shift_dtype, m.shift + at);
     }
     int flip = 0;
     float v[1][8];
@@ -644,8 +645,10 @@ __global__ void __launch_bounds__(1024) gated_norm_row_kernel(const __grid_const
         values8<XT>(xr[0], v[0]);
     }
     if (a.h == nullptr) return;
-    RawAny weight, bias;
+    RawAny weight, bias, scale, shift;                                        // on their way during the sums
     if (in) {
+        load_any(scale, a.scale, a.scale_dtype, m.scale + at);
+        load_any(shift, a.shift, a.shift_dtype, m.shift + at);
         load_any(weight, a.weight, a.weight_dtype, at);
         load_any(bias, a.bias, a.bias_dtype, at);
     }
@@ -682,15 +685,34 @@ __device__ __forceinline__ void load_elements(uint32_t (&r)[NE], const void* bas
             if (i < count) r[i] = __ldg(q + i * step);
     }
 }
-__device__ __forceinline__ float element(uint32_t r, int type) {
-    if (type == FEATHER_SRC_FP32) return __uint_as_float(r);
-    if (type == FEATHER_SRC_BF16) return __uint_as_float(r << 16);
-    return __half2float(__ushort_as_half(static_cast<uint16_t>(r)));
+// The type is looked at once for a thread's elements, not for each.
+template <int NE, typename Op>
+__device__ __forceinline__ void each_element(const uint32_t (&r)[NE], int type, Op op) {
+    if (type == FEATHER_SRC_FP32) {
+#pragma unroll
+        for (int i = 0; i < NE; ++i) op(i, __uint_as_float(r[i]));
+    } else if (type == FEATHER_SRC_BF16) {
+#pragma unroll
+        for (int i = 0; i < NE; ++i) op(i, __uint_as_float(r[i] << 16));
+    } else {
+#pragma unroll
+        for (int i = 0; i < NE; ++i) op(i, __half2float(__ushort_as_half(static_cast<uint16_t>(r[i]))));
+    }
 }
-__device__ __forceinline__ void store_element(void* base, int type, long long at, float v) {
-    if (type == FEATHER_SRC_FP32) static_cast<float*>(base)[at] = v;
-    else if (type == FEATHER_SRC_BF16) static_cast<__nv_bfloat16*>(base)[at] = __float2bfloat16_rn(v);
-    else static_cast<__half*>(base)[at] = __float2half_rn(v);
+template <int NE>
+__device__ __forceinline__ void store_elements(void* base, int type, long long at, int step, int count, const float (&v)[NE]) {
+    if (type == FEATHER_SRC_FP32) {
+        float* const o = static_cast<float*>(base) + at;
+#pragma unroll
+        for (int i = 0; i < NE; ++i)
+            if (i < count) o[i * step] = v[i];
+    } else {
+        uint16_t* const o = static_cast<uint16_t*>(base) + at;
+        const bool bf16 = type == FEATHER_SRC_BF16;
+#pragma unroll
+        for (int i = 0; i < NE; ++i)
+            if (i < count) o[i * step] = static_cast<uint16_t>(pack16x2(v[i], 0.0f, bf16));
+    }
 }
 
 template <int NE>
@@ -710,9 +732,9 @@ __device__ __forceinline__ float normalise_elements(float (&v)[NE], const NormPa
     return 1.0f / sqrtf(row_sum<false>(s, part, flip) * p.inv_cols + p.a.eps);
 }
 
-// EARLY: every operand of the row is loaded before the first one is used (eight registers an element); otherwise each where it is used.
+// EARLY: what makes r is loaded together, what makes h of it before the second norm's sums; otherwise each where it is used.
 template <int NE, bool EARLY>
-__global__ void __launch_bounds__(EARLY ? 512 : 1024) gated_norm_elements_kernel(const NormParams p) {
+__global__ void __launch_bounds__(EARLY ? 512 : 1024) gated_norm_elements_kernel(const __grid_constant__ NormParams p) {
     __shared__ __align__(16) float part[2][kNormMaxWarps];
     const feather_norm_args& a = p.a;
     clear_parts(part);
@@ -722,9 +744,8 @@ __global__ void __launch_bounds__(EARLY ? 512 : 1024) gated_norm_elements_kernel
     const int t = threadIdx.x, step = blockDim.x;
     const int count = p.vecs > t ? min(NE, (p.vecs - t + step - 1) / step) : 0;
     int flip = 0;
-    const long long gate_at = (a.gate != nullptr ? row / a.gate_rows * a.gate_ld : 0) + t;
-    const long long scale_at = (a.scale != nullptr ? row / a.scale_rows * a.scale_ld : 0) + t;
-    const long long shift_at = (a.shift != nullptr ? row / a.shift_rows * a.shift_ld : 0) + t;
+    const ModulationAt m = modulation_at(a, row);
+    const long long gate_at = m.gate + t, scale_at = m.scale + t, shift_at = m.shift + t;
     uint32_t x[NE], y[NE], gate[NE], post_weight[NE], weight[NE], bias[NE], scale[NE], shift[NE];
     load_elements<NE>(x, a.x, a.x_dtype, row * a.ldx + t, step, count);
     load_elements<NE>(y, a.y, a.y_dtype, row * a.ldy + t, step, count);
@@ -732,50 +753,41 @@ __global__ void __launch_bounds__(EARLY ? 512 : 1024) gated_norm_elements_kernel
         load_elements<NE>(gate, a.gate, a.gate_dtype, gate_at, step, count);
         load_elements<NE>(post_weight, a.post_weight, a.post_weight_dtype, t, step, count);
     };
+    if (EARLY) load_before();
+    float v[NE];                                                              // elements past the row are zero until the sums are done
+    if (a.y != nullptr) {
+        each_element<NE>(y, a.y_dtype, [&](int i, float e) { v[i] = i < count ? e : 0.0f; });
+        const float inv = a.post_norm ? normalise_elements<NE>(v, p, count, part, flip) : 1.0f;
+        if (!EARLY) load_before();
+#pragma unroll
+        for (int i = 0; i < NE; ++i) v[i] *= inv * a.residual_scale;
+        if (a.gate != nullptr) each_element<NE>(gate, a.gate_dtype, [&](int i, float e) { v[i] *= e; });
+        if (a.post_weight != nullptr) each_element<NE>(post_weight, a.post_weight_dtype, [&](int i, float e) { v[i] *= e; });
+        each_element<NE>(x, a.x_dtype, [&](int i, float e) { v[i] = i < count ? v[i] + e : 0.0f; });
+        if (a.r != nullptr) store_elements<NE>(a.r, a.x_dtype, row * a.ldr + t, step, count, v);
+    } else {
+        each_element<NE>(x, a.x_dtype, [&](int i, float e) { v[i] = i < count ? e : 0.0f; });
+    }
+    if (a.h == nullptr) return;
     if (EARLY) {
-        load_before();
         load_elements<NE>(weight, a.weight, a.weight_dtype, t, step, count);
         load_elements<NE>(bias, a.bias, a.bias_dtype, t, step, count);
         load_elements<NE>(scale, a.scale, a.scale_dtype, scale_at, step, count);
         load_elements<NE>(shift, a.shift, a.shift_dtype, shift_at, step, count);
     }
-    float v[NE];
-    if (a.y != nullptr) {
-#pragma unroll
-        for (int i = 0; i < NE; ++i) v[i] = i < count ? element(y[i], a.y_dtype) : 0.0f;
-        const float inv = a.post_norm ? normalise_elements<NE>(v, p, count, part, flip) : 1.0f;
-        if (!EARLY) load_before();
-#pragma unroll
-        for (int i = 0; i < NE; ++i) {
-            if (i >= count) continue;
-            float g = a.residual_scale;
-            if (a.gate != nullptr) g *= element(gate[i], a.gate_dtype);
-            if (a.post_weight != nullptr) g *= element(post_weight[i], a.post_weight_dtype);
-            v[i] = element(x[i], a.x_dtype) + g * (v[i] * inv);
-            if (a.r != nullptr) store_element(a.r, a.x_dtype, row * a.ldr + t + i * step, v[i]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < NE; ++i) v[i] = i < count ? element(x[i], a.x_dtype) : 0.0f;
-    }
-    if (a.h == nullptr) return;
     const float inv = normalise_elements<NE>(v, p, count, part, flip);
+#pragma unroll
+    for (int i = 0; i < NE; ++i) v[i] *= inv;
     const auto apply = [&](uint32_t(&r)[NE], const void* base, int type, long long at, auto op) {
         if (base == nullptr) return;
         if (!EARLY) load_elements<NE>(r, base, type, at, step, count);
-#pragma unroll
-        for (int i = 0; i < NE; ++i)
-            if (i < count) v[i] = op(v[i], element(r[i], type));
+        each_element<NE>(r, type, op);
     };
-#pragma unroll
-    for (int i = 0; i < NE; ++i) v[i] *= inv;
-    apply(weight, a.weight, a.weight_dtype, t, [](float u, float m) { return u * m; });
-    apply(bias, a.bias, a.bias_dtype, t, [](float u, float m) { return u + m; });
-    apply(scale, a.scale, a.scale_dtype, scale_at, [](float u, float m) { return u * (1.0f + m); });
-    apply(shift, a.shift, a.shift_dtype, shift_at, [](float u, float m) { return u + m; });
-#pragma unroll
-    for (int i = 0; i < NE; ++i)
-        if (i < count) store_element(a.h, a.h_dtype, row * a.ldh + t + i * step, v[i]);
+    apply(weight, a.weight, a.weight_dtype, t, [&](int i, float e) { v[i] *= e; });
+    apply(bias, a.bias, a.bias_dtype, t, [&](int i, float e) { v[i] += e; });
+    apply(scale, a.scale, a.scale_dtype, scale_at, [&](int i, float e) { v[i] *= 1.0f + e; });
+    apply(shift, a.shift, a.shift_dtype, shift_at, [&](int i, float e) { v[i] += e; });
+    store_elements<NE>(a.h, a.h_dtype, row * a.ldh + t, step, count, v);
 }
 
 // ------------------------------------------------------------------------------------------------ launches
@@ -880,7 +892,9 @@ static cudaError_t norm_launch_typed(const NormParams& p, int sms, cudaStream_t 
     // A block for each row up to two waves of them (16 of narrow rows: 2080 x 1024 fp32 7.8 us against 8.6 us, 1000 x 5120 27 us against 17 us),
     // and where every row has a modulation of its own.
     if (p.vecs <= 1024 && (shared < 4 || a.rows <= (p.vecs <= 128 ? 16 : 2) * sms))
-        return norm_launch_kernel(gated_norm_row_kernel<XT, YT>, a.rows, (p.vecs + 31) / 32 * 32, 0, stream, p);
+        return a.rows > 2 * sms && p.vecs > 512
+                   ? norm_launch_kernel(gated_norm_row_kernel<XT, YT, true>, a.rows, (p.vecs + 31) / 32 * 32, 0, stream, p)
+                   : norm_launch_kernel(gated_norm_row_kernel<XT, YT, false>, a.rows, (p.vecs + 31) / 32 * 32, 0, stream, p);
     if (p.vecs <= 32) return norm_launch_groups<XT, YT, 1>(p, sms, shared >= 4, stream);
     return p.vecs <= 64 ? norm_launch_groups<XT, YT, 2>(p, sms, shared >= 4, stream) : norm_launch_groups<XT, YT, 4>(p, sms, shared >= 4, stream);
 }
@@ -936,6 +950,9 @@ extern "C" int feather_gated_norm(const feather_norm_args* args_host, feather_st
     const bool packed = a.h != nullptr && a.h_scales != nullptr;
     if ((a.gate != nullptr && a.gate_rows <= 0) || (a.scale != nullptr && a.scale_rows <= 0) || (a.shift != nullptr && a.shift_rows <= 0))
         return set_error(FEATHER_ERR_BAD_ARGUMENT, "gate_rows, scale_rows and shift_rows must be positive");
+    a.gate_rows = a.gate_rows < a.rows ? a.gate_rows : a.rows;                 // 31 bits
+    a.scale_rows = a.scale_rows < a.rows ? a.scale_rows : a.rows;
+    a.shift_rows = a.shift_rows < a.rows ? a.shift_rows : a.rows;
     bool vector = a.cols % 8 == 0;
     bool ok = norm_operand(a.x, a.x_dtype, a.ldx, a.rows, a.cols, &vector) && norm_operand(a.y, a.y_dtype, a.ldy, a.rows, a.cols, &vector) &&
               norm_operand(a.r, a.x_dtype, a.ldr, a.rows, a.cols, &vector) && norm_operand(a.weight, a.weight_dtype, 0, 1, a.cols, &vector) &&

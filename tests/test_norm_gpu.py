@@ -178,3 +178,19 @@ def test_empty_and_graph(norm, cuda_dev):
         got = norm.gated_residual_norm(x, y, post_norm=True)
     s.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
+@pytest.mark.parametrize("cols", [256, 1000, 4104, 5120, 8192, 12288])
+@pytest.mark.parametrize("x_dtype", [BF16, FP32])
+def test_a_modulation_for_each_row(norm, mx, cuda_dev, cols, x_dtype):
+    shape = (2, 210, cols)
+    x, y = _t(shape, 1, cuda_dev, x_dtype), _t(shape, 2, cuda_dev, BF16)
+    shift, scale, gate = (t for t in _t((2, 210, 3 * cols), 3, cuda_dev, spread=0.3).chunk(3, dim=-1))
+    kw = dict(gate=gate, scale=scale, shift=shift, post_norm=True, post_weight=_t((cols,), 4, cuda_dev, BF16, 0.2, 1.0), weight=_t((cols,), 5, cuda_dev, FP16, 0.2, 1.0), bias=_t((cols,), 6, cuda_dev))
+    for kind in ("rms", "layer"):
+        _check(norm, x, y, kind=kind, **kw)
+    if cols % 32 == 0:
+        _, h = norm.gated_residual_norm(x, y, out_dtype=BF16, **kw)
+        _, (data, scales) = norm.gated_residual_norm(x, y, out_dtype=BF16, packed=True, **kw)
+        ref_data, ref_scales = mx.quantize_mxfp4(h.view(-1, cols))
+        assert torch.equal(data, ref_data) and torch.equal(mx.unprepack_mxfp4_scales(scales, 420, cols), mx.unprepack_mxfp4_scales(ref_scales, 420, cols))
