@@ -306,11 +306,12 @@ __device__ __forceinline__ void join8(const float (&f)[8], F2 (&v)[4]) {
 // lie in shared memory, once for the block, and are folded anew where a wave begins that belongs to other rows of gate, scale or shift
 // (a wave ends there).
 // Bound by the instructions around the arithmetic rather than by memory: 2 x 8192 x 5120 bf16 with fp32 gate, scale and shift of each
-// sample takes 142 us as layer norm (4.7 TB/s of 671 MB) and 114 us as rms norm with a weight (5.9 TB/s); a block for each row that
-// reads its vectors from the cache takes 213 and 136 us.
+// sample takes 127 us as layer norm (5.3 TB/s of 671 MB), 154 us as a packed result, 185 us with a norm of y before it; a block for each
+// row that reads its vectors from the cache takes 213 us for the first.
 constexpr int kNormMaxStages = 4, kNormMaxGroups = 32, kNormMaxBarriers = 15;    // a group of one warp needs no barrier
-// Registers of a thread.
-__host__ __device__ constexpr int norm_regs(int nv) { return nv == 4 ? 128 : nv == 2 ? 96 : 64; }
+// Registers of a thread.  POST: y may go through a norm first, and x has to wait for it in registers.  Without that norm r is formed as x
+// and y are read, 96 registers are enough, and 640 columns in eights have four groups instead of three (127 us where 128 registers take 141).
+__host__ __device__ constexpr int norm_regs(int nv, bool post) { return nv == 4 && post ? 128 : nv == 1 ? 64 : 96; }
 
 struct GroupBarrier {
     int id, threads;
@@ -322,7 +323,7 @@ struct GroupBarrier {
 
 // A group's place for its warps' partial sums: two buffers in turn, so that one barrier for each sum is enough.
 struct GroupSums {
-    float2 (*part)[kNormMaxWarps];
+    float2* part;                                                             // the second buffer kNormMaxWarps further on
     const float* elements;                                                    // of the row in each warp
     int warps, warp, flip;
 };
@@ -367,7 +368,7 @@ __device__ __forceinline__ float normalise_group(F2 (&v)[NV][4], const NormParam
     f2_split(q, lo, hi);
     float squares = total(lo + hi);
     if (sums.warps > 1) {
-        float2* const part = sums.part[sums.flip];
+        float2* const part = sums.part + sums.flip * kNormMaxWarps;
         sums.flip ^= 1;
         if ((threadIdx.x & 31) == 0) part[sums.warp] = make_float2(mean, squares);
         barrier.sync();
@@ -389,9 +390,9 @@ __device__ __forceinline__ float normalise_group(F2 (&v)[NV][4], const NormParam
     return 1.0f / sqrtf(squares * p.inv_cols + p.a.eps);
 }
 
-template <int XT, int YT, int NV, bool KEEP, bool FULL>
-__global__ void __maxnreg__(norm_regs(NV)) gated_norm_groups_kernel(const __grid_constant__ NormParams p) {
-    __shared__ float2 part[kNormMaxBarriers][2][kNormMaxWarps];
+template <int XT, int YT, int NV, bool KEEP, bool FULL, bool POST>
+__global__ void __maxnreg__(norm_regs(NV, POST)) gated_norm_groups_kernel(const __grid_constant__ NormParams p) {
+    __shared__ float2 part[2][kNormMaxWarps];                                 // by the block's warps
     __shared__ float elements[kNormMaxWarps];
     __shared__ __align__(8) uint64_t bars[kNormMaxGroups][kNormMaxStages];
     __shared__ int abort_flag;
@@ -422,7 +423,7 @@ __global__ void __maxnreg__(norm_regs(NV)) gated_norm_groups_kernel(const __grid
     pdl_launch_dependents();
     pdl_wait_for_previous_kernel();
     const GroupBarrier barrier{1 + group, step};
-    GroupSums sums{part[group < kNormMaxBarriers ? group : 0], elements, step / 32, t / 32, 0};
+    GroupSums sums{part[0] + group * (step / 32), elements, step / 32, t / 32, 0};
     const long long begin = static_cast<long long>(blockIdx.x) * p.chunk, end = begin + p.chunk < a.rows ? begin + p.chunk : a.rows;
     // A wave: rows wave .. wave + groups - 1, one a group, short of the next change of coefficients.
     long long fetch_wave = begin, fetch_change = begin;
@@ -499,15 +500,41 @@ __global__ void __maxnreg__(norm_regs(NV)) gated_norm_groups_kernel(const __grid
             v[2] = f2(y.x, y.y);
             v[3] = f2(y.z, y.w);
         };
-        Raw8<XT> xr[NV];
+        const auto residual = [&](int i, const Raw8<XT>& x_raw, F2(&y)[4], F2 by) {  // r of one vector, in y's place
+            const int vec = t + i * step;
+            F2 g[4], x[4];
+            float f[8];
+            if (!(present & kNormG)) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) g[j] = f2(a.residual_scale, a.residual_scale);
+            } else if constexpr (KEEP) {
+                coefficient(0, vec, g);
+            } else {
+                RawAny q, w;
+                load_any(q, a.gate, a.gate_dtype, m.gate + vec * 8);
+                load_any(w, a.post_weight, a.post_weight_dtype, vec * 8);
+                fold_g(a, q, w, f);
+                join8(f, g);
+            }
+            values8<XT>(x_raw, x);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = f2_fma(g[j], POST ? f2_mul(y[j], by) : y[j], x[j]);
+            if (a.r != nullptr) {
+                split8(y, f);
+                store8<XT>(a.r, row * a.ldr + vec * 8, f);
+            }
+        };
+        Raw8<XT> xr[POST ? NV : 1];
         F2 v[NV][4];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int vec = t + i * step;
             if (FULL || vec < p.vecs) {
-                xr[i] = reinterpret_cast<const Raw8<XT>*>(from)[vec];
+                Raw8<XT>& x = xr[POST ? i : 0];
+                x = reinterpret_cast<const Raw8<XT>*>(from)[vec];
                 if (has_y) values8<YT>(reinterpret_cast<const Raw8<YT>*>(from + x_bytes)[vec], v[i]);
-                else values8<XT>(xr[i], v[i]);
+                else values8<XT>(x, v[i]);
+                if (!POST && has_y) residual(i, x, v[i], F2{});
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[i][j] = f2(0.0f, 0.0f);
@@ -515,34 +542,13 @@ __global__ void __maxnreg__(norm_regs(NV)) gated_norm_groups_kernel(const __grid
         }
         barrier.sync();                                                       // every thread has its part in registers
         if (t == 0) fetch();
-        if (has_y) {
-            const float inv = a.post_norm ? normalise_group<NV, FULL>(v, p, t, step, barrier, sums) : 1.0f;
-            const F2 by = f2(inv, inv);
+        if constexpr (POST) {
+            if (has_y) {
+                const float inv = a.post_norm ? normalise_group<NV, FULL>(v, p, t, step, barrier, sums) : 1.0f;
+                const F2 by = f2(inv, inv);
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int vec = t + i * step;
-                if (!FULL && vec >= p.vecs) continue;
-                F2 g[4], x[4];
-                float f[8];
-                if (!(present & kNormG)) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) g[j] = f2(a.residual_scale, a.residual_scale);
-                } else if constexpr (KEEP) {
-                    coefficient(0, vec, g);
-                } else {
-                    RawAny q, w;
-                    load_any(q, a.gate, a.gate_dtype, m.gate + vec * 8);
-                    load_any(w, a.post_weight, a.post_weight_dtype, vec * 8);
-                    fold_g(a, q, w, f);
-                    join8(f, g);
-                }
-                values8<XT>(xr[i], x);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[i][j] = f2_fma(g[j], f2_mul(v[i][j], by), x[j]);
-                if (a.r != nullptr) {
-                    split8(v[i], f);
-                    store8<XT>(a.r, row * a.ldr + vec * 8, f);
-                }
+                for (int i = 0; i < NV; ++i)
+                    if (FULL || t + i * step < p.vecs) residual(i, xr[i], v[i], by);
             }
         }
         if (a.h == nullptr) continue;
@@ -801,7 +807,7 @@ static int norm_sm_count() {
     return cached[dev];
 }
 
-constexpr int kNormMaxSmem = 216 * 1024;      // dynamic, beside the 8 KB of sums and barriers
+constexpr int kNormMaxSmem = 225 * 1024;      // dynamic, beside the sums and barriers
 
 template <typename... Params, typename... Args>
 static cudaError_t norm_launch_kernel(void (*kernel)(Params...), long long grid, int threads, int smem, cudaStream_t stream, const Args&... args) {
@@ -847,26 +853,31 @@ struct NormOccupancy {
 // Consecutive rows of each resident block.
 static int norm_chunk(int64_t rows, int64_t units) { return static_cast<int>((rows + units - 1) / units); }
 
-template <int XT, int YT, int NV, bool KEEP, bool FULL>
+template <int XT, int YT, int NV, bool KEEP, bool FULL, bool POST>
 static cudaError_t norm_launch_groups_kernel(NormParams p, int threads, int smem, int sms, cudaStream_t stream) {
     static NormOccupancy occupancy;
     int blocks;
-    const cudaError_t e = occupancy.get(gated_norm_groups_kernel<XT, YT, NV, KEEP, FULL>, smem / 1024, threads * p.groups, smem, &blocks);
+    const cudaError_t e = occupancy.get(gated_norm_groups_kernel<XT, YT, NV, KEEP, FULL, POST>, smem / 1024, threads * p.groups, smem, &blocks);
     if (e != cudaSuccess) return e;
     p.chunk = norm_chunk(p.a.rows, static_cast<int64_t>(blocks) * sms);
-    return norm_launch_kernel(gated_norm_groups_kernel<XT, YT, NV, KEEP, FULL>, (p.a.rows + p.chunk - 1) / p.chunk, threads * p.groups, smem, stream, p);
+    return norm_launch_kernel(gated_norm_groups_kernel<XT, YT, NV, KEEP, FULL, POST>, (p.a.rows + p.chunk - 1) / p.chunk, threads * p.groups, smem, stream, p);
 }
 
-template <int XT, int YT, int NV>
+template <int XT, int YT>
+static int norm_row_bytes(const feather_norm_args& a) {
+    return static_cast<int>(a.cols) * ((XT == FEATHER_SRC_FP32 ? 4 : 2) + (a.y == nullptr ? 0 : YT == FEATHER_SRC_FP32 ? 4 : 2));
+}
+
+template <int XT, int YT, int NV, bool POST>
 static cudaError_t norm_launch_groups(NormParams p, int sms, bool shared, cudaStream_t stream) {
     const int threads = (p.vecs + 32 * NV - 1) / (32 * NV) * 32;
-    const int row_bytes = static_cast<int>(p.a.cols) * ((XT == FEATHER_SRC_FP32 ? 4 : 2) + (p.a.y == nullptr ? 0 : YT == FEATHER_SRC_FP32 ? 4 : 2));
+    const int row_bytes = norm_row_bytes<XT, YT>(p.a);
     const int kept = norm_present(p.a) != 0 ? 3 * 32 * p.vecs : 0;
     // One block an SM.  As many groups as its registers hold, each with two rows of ring at least; the coefficients stay in shared memory
     // if one group's row fits beside them.
     const bool keep = shared && kept + row_bytes <= kNormMaxSmem;
     const int room = kNormMaxSmem - (keep ? kept : 0);
-    p.groups = 65536 / norm_regs(NV) / 128 * 128 / threads;                   // registers go to four warps at a time
+    p.groups = 65536 / norm_regs(NV, POST) / 128 * 128 / threads;             // registers go to four warps at a time
     if (threads > 32 && p.groups > kNormMaxBarriers) p.groups = kNormMaxBarriers;
     if (p.groups * threads > 1024) p.groups = 1024 / threads;
     while (p.groups > 1 && p.groups * 2 * row_bytes > room) --p.groups;
@@ -875,10 +886,11 @@ static cudaError_t norm_launch_groups(NormParams p, int sms, bool shared, cudaSt
     if (p.stages > kNormMaxStages) p.stages = kNormMaxStages;
     if (p.stages < 1) return cudaErrorInvalidConfiguration;
     const int smem = (keep ? kept : 0) + p.groups * p.stages * row_bytes;
-    if constexpr (NV == 4)
-        if (!keep) return norm_launch_groups_kernel<XT, YT, NV, false, false>(p, threads, smem, sms, stream);
-    return p.vecs == threads * NV ? norm_launch_groups_kernel<XT, YT, NV, true, true>(p, threads, smem, sms, stream)
-                                  : norm_launch_groups_kernel<XT, YT, NV, true, false>(p, threads, smem, sms, stream);
+    if (!keep && !(NV == 4 && POST)) return cudaErrorInvalidConfiguration;
+    if constexpr (NV == 4 && POST)
+        if (!keep) return norm_launch_groups_kernel<XT, YT, NV, false, false, POST>(p, threads, smem, sms, stream);
+    return p.vecs == threads * NV ? norm_launch_groups_kernel<XT, YT, NV, true, true, POST>(p, threads, smem, sms, stream)
+                                  : norm_launch_groups_kernel<XT, YT, NV, true, false, POST>(p, threads, smem, sms, stream);
 }
 
 template <int XT, int YT>
@@ -895,8 +907,15 @@ static cudaError_t norm_launch_typed(const NormParams& p, int sms, cudaStream_t 
         return a.rows > 2 * sms && p.vecs > 512
                    ? norm_launch_kernel(gated_norm_row_kernel<XT, YT, true>, a.rows, (p.vecs + 31) / 32 * 32, 0, stream, p)
                    : norm_launch_kernel(gated_norm_row_kernel<XT, YT, false>, a.rows, (p.vecs + 31) / 32 * 32, 0, stream, p);
-    if (p.vecs <= 32) return norm_launch_groups<XT, YT, 1>(p, sms, shared >= 4, stream);
-    return p.vecs <= 64 ? norm_launch_groups<XT, YT, 2>(p, sms, shared >= 4, stream) : norm_launch_groups<XT, YT, 4>(p, sms, shared >= 4, stream);
+    if (p.vecs <= 32) return norm_launch_groups<XT, YT, 1, true>(p, sms, shared >= 4, stream);
+    if (p.vecs <= 64) return norm_launch_groups<XT, YT, 2, true>(p, sms, shared >= 4, stream);
+    // The form without a norm of y, for the pairs of types that models have; it has its coefficients in shared memory always, and above 1536
+    // vectors 96 registers give no further group (16384 rows of 6144: 95 -> 79 us, 8192: 153 -> 113 us; fp32 2 x 2048 x 5120 127 -> 96 us;
+    // an rms norm with a weight alone, which is nearest to the memory's rate, loses 123 -> 128 us).
+    if constexpr (XT == YT || XT == FEATHER_SRC_FP32)
+        if (!a.post_norm && shared >= 4 && p.vecs <= 1536 && 96 * p.vecs + norm_row_bytes<XT, YT>(a) <= kNormMaxSmem)
+            return norm_launch_groups<XT, YT, 4, false>(p, sms, true, stream);
+    return norm_launch_groups<XT, YT, 4, true>(p, sms, shared >= 4, stream);
 }
 
 static cudaError_t norm_launch(const NormParams& p, int sms, cudaStream_t stream) {

@@ -92,6 +92,19 @@ def test_thousands_of_rows_of_other_types(norm, cuda_dev, x_dtype, y_dtype):
         _check(norm, wide[:, 8:-8], y.view(-1, cols), residual_scale=0.25)
 
 
+@pytest.mark.parametrize("x_dtype,y_dtype", [(BF16, BF16), (FP16, FP16), (FP32, FP32), (FP32, BF16), (FP16, BF16)])
+def test_thousands_of_rows_without_a_norm_of_y(norm, cuda_dev, x_dtype, y_dtype):
+    """Nothing waits for y's statistics: both sides of the widths and of the shared memory where the form for it ends (12288 fp32 columns
+    with coefficients are too many, without them they are not)."""
+    for cols in (520, 1536, 5120, 6144, 12288, 12296):
+        x, y = _t((3, 701, cols), 1, cuda_dev, x_dtype, about=0.5), _t((3, 701, cols), 2, cuda_dev, y_dtype)
+        for kind in ("rms", "layer"):
+            _check(norm, x, y, gate=_t((3, 1, cols), 3, cuda_dev), scale=_t((3, 1, cols), 4, cuda_dev, spread=0.2), shift=_t((cols,), 5, cuda_dev), kind=kind)
+        _check(norm, x, y, residual_scale=0.25, weight=_t((cols,), 7, cuda_dev, FP16, 0.2, 1.0), kind="rms")
+        _check(norm, x, y, kind="layer")
+        _check(norm, x, None, bias=_t((cols,), 8, cuda_dev), kind="layer")
+
+
 @pytest.mark.parametrize("x_dtype", [BF16, FP16, FP32])
 @pytest.mark.parametrize("y_dtype", [BF16, FP16, FP32])
 def test_types(norm, cuda_dev, x_dtype, y_dtype):
