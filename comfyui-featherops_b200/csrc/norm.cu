@@ -310,7 +310,7 @@ __device__ __forceinline__ void join8(const float (&f)[8], F2 (&v)[4]) {
 // row that reads its vectors from the cache takes 213 us for the first.
 constexpr int kNormMaxStages = 4, kNormMaxGroups = 32, kNormMaxBarriers = 15;    // a group of one warp needs no barrier
 // Registers of a thread.  POST: y may go through a norm first, and x has to wait for it in registers.  Without that norm r is formed as x
-// and y are read, 96 registers are enough, and 640 columns in eights have four groups instead of three (127 us where 128 registers take 141).
+// and y are read, 96 registers are enough, and rows of 5120 have four groups instead of three (127 us where 128 registers take 141).
 __host__ __device__ constexpr int norm_regs(int nv, bool post) { return nv == 4 && post ? 128 : nv == 1 ? 64 : 96; }
 
 struct GroupBarrier {
