@@ -1,7 +1,7 @@
 // MXFP4 weight and activation format: quantise rows of fp32 / bf16 / fp16 and the inverse.  The format is in mxfp4.cuh.
 //
-// Both are byte movers.  A lane holds eight elements, four lanes a block of 32, so the block's maximum is two shuffles and all
-// loads and stores are whole 16-byte vectors; nothing is staged and every byte is touched once.
+// Both are byte movers.  A lane holds eight elements, four lanes a block of 32 (16 and two for aligned 16-bit sources), so the block's
+// maximum is a shuffle or two and all loads and stores are whole vectors; nothing is staged and every byte is touched once.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -14,9 +14,9 @@ namespace feather {
 
 constexpr int kMxThreads = 256;
 
-// Rows of a thread where there are rows enough: loads under way against registers.  One, two, four and eight rows take 36, 31, 30, 33 us to
-// quantise 4096 x 13824 bf16 (143 MB; 30 us is 4.8 TB/s, bound by the conversions) and 54, 49, 50, 71 us for 13824 x 5120 fp32 (49 us is
-// 6.5 TB/s, a copy's rate); dequantising 33, 26, 25, 25 us and 70, 69, 72, 74 us (the rate at which memory is written).
+// Rows of a thread where there are rows enough: loads under way against registers.  One, two, four and eight rows take 54, 49, 50, 71 us to
+// quantise 13824 x 5120 fp32 (48 us now, 6.7 TB/s, a copy's rate) and 36, 31, 30, 33 us for 4096 x 13824 bf16; dequantising 4096 x 13824 bf16 33, 26, 25, 25 us and 13824 x 5120 fp32 70,
+// 69, 72, 74 us (the rate at which memory is written).
 __host__ __device__ constexpr int mx_many_rows(int type) { return type == FEATHER_SRC_FP32 ? 2 : 4; }
 
 // Eight elements as they lie in memory; 16-bit ones two to a word.  kVector: p is 16-byte aligned.
@@ -55,6 +55,13 @@ __device__ __forceinline__ void mx_values8(const MxRaw<kSrc>& r, float (&x)[8]) 
     }
 }
 
+// fp32 bits of the larger of two 16-bit |x|.
+template <int kSrc>
+__device__ __forceinline__ uint32_t mx_top16(uint32_t pair) {
+    const uint32_t top = max(pair >> 16, pair & 0xFFFFu);
+    return kSrc == FEATHER_SRC_BF16 ? top << 16 : __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(top))));
+}
+
 // fp32 bits of the largest |x| of the block that four neighbouring lanes hold.  16-bit values are compared as they are, two a word: their
 // bits order like the values too.
 template <int kSrc>
@@ -70,8 +77,7 @@ __device__ __forceinline__ uint32_t mx_block_top(const MxRaw<kSrc>& r) {
         for (int i = 0; i < 4; ++i) top = __vmaxu2(top, r.w[i] & 0x7FFF7FFFu);
         top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        top = max(top >> 16, top & 0xFFFFu);
-        return kSrc == FEATHER_SRC_BF16 ? top << 16 : __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(top))));
+        return mx_top16<kSrc>(top);
     }
 }
 
@@ -105,6 +111,47 @@ mx_quantize_kernel(const void* __restrict__ src, long long rows, int k, long lon
             reinterpret_cast<uint32_t*>(data)[row * (k / 8) + vec] = q;
             if ((vec & 15) == 0) *reinterpret_cast<uint32_t*>(scales + mx_scale_word_offset(row, vec >> 4, mx_tiles_k(k))) = word;
         }
+    }
+}
+
+// 16-bit sources: a lane holds 16 elements, two lanes a block, so that what a block costs (shuffles, the scale, addresses) is shared by
+// twice as many: the instructions bound this, not the bytes.  4096 x 13824 bf16 takes 23.5 us (143 MB, 6.1 TB/s) and 30.2 us with eight a
+// lane, 1024 x 5120 3.9 and 4.9 us.  tx is a multiple of 8 (four blocks sit in a quarter-warp); src and its rows are 32-byte aligned.
+template <int kSrc>
+__global__ void __launch_bounds__(kMxThreads)
+mx_quantize16_kernel(const uint16_t* __restrict__ src, long long rows, int k, long long ld, uint8_t* __restrict__ data, uint8_t* __restrict__ scales) {
+    pdl_launch_dependents();
+    pdl_wait_for_previous_kernel();
+    const long long row = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y;
+    const int vec = blockIdx.y * blockDim.x + threadIdx.x;
+    const int lane = (threadIdx.y * blockDim.x + threadIdx.x) & 31;
+    const bool in = vec * 16 < k;
+    const uint16_t* const from = src + row * ld + vec * 16;
+    uint32_t raw[8] = {};
+    if (in && row < rows)
+        asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(raw[0]), "=r"(raw[1]), "=r"(raw[2]), "=r"(raw[3]), "=r"(raw[4]), "=r"(raw[5]), "=r"(raw[6]), "=r"(raw[7])
+                     : "l"(from));
+    uint2* const to = reinterpret_cast<uint2*>(data) + row * (k / 16) + vec;
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = __vmaxu2(top, raw[i] & 0x7FFF7FFFu);
+    top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    const uint32_t code = mx_code(mx_top16<kSrc>(top));
+    uint32_t q[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) unpack16x2(raw[4 * h + i], kSrc == FEATHER_SRC_BF16, x[2 * i], x[2 * i + 1]);
+        q[h] = mx_scaled_pack8(x, code);
+    }
+    uint32_t word = code << (8 * ((lane >> 1) & 3));
+    word |= __shfl_xor_sync(0xffffffffu, word, 2);
+    word |= __shfl_xor_sync(0xffffffffu, word, 4);
+    if (in && row < rows) {
+        *to = make_uint2(q[0], q[1]);
+        if ((vec & 7) == 0) *reinterpret_cast<uint32_t*>(scales + mx_scale_word_offset(row, vec >> 3, mx_tiles_k(k))) = word;
     }
 }
 
@@ -156,12 +203,15 @@ static int mx_check(int64_t rows, int64_t K) {
     return FEATHER_OK;
 }
 
-// (tx, ty) and grid: the narrowest power of two that covers a row's 8-element vectors, at most a whole block.  *many: rows enough for
-// threads of mx_many_rows rows, whose grid still fills the SMs twice over.
-static void mx_grid(int64_t rows, int64_t K, int many_rows, bool vector, dim3* grid, dim3* block, bool* many) {
-    unsigned tx = 16;
-    while (tx < kMxThreads && tx * 8 < K) tx <<= 1;
-    const unsigned ty = kMxThreads / tx, along = static_cast<unsigned>((K / 8 + tx - 1) / tx);
+// (tx, ty) and grid: the narrowest power of two that covers a row's vectors, at most a whole block, and less where that leaves over a
+// sixteenth of the lanes idle (8192 x 5120 bf16: 21.7 -> 17.2 us).  *many: rows enough for threads of many_rows rows, whose grid still
+// fills the SMs twice over.
+static void mx_grid(int64_t rows, int64_t K, int elements, int many_rows, bool vector, dim3* grid, dim3* block, bool* many) {
+    const int64_t lanes = K / elements;
+    unsigned tx = 128 / elements;
+    while (tx < kMxThreads && tx < lanes) tx <<= 1;
+    while (tx > 32 && ((lanes + tx - 1) / tx * tx - lanes) * 16 > lanes) tx >>= 1;
+    const unsigned ty = kMxThreads / tx, along = static_cast<unsigned>((lanes + tx - 1) / tx);
     *many = vector && (rows + ty * many_rows - 1) / (ty * many_rows) * along >= 2 * 148 * 8;
     const unsigned step = *many ? ty * many_rows : ty;
     *block = dim3(tx, ty, 1);
@@ -217,9 +267,15 @@ extern "C" int feather_mxfp4_quantize(const void* src, int src_dtype, int64_t ro
     const bool vector = mx_aligned16(src) && (rows == 1 || ld * size % 16 == 0);
     dim3 grid, block;
     bool many;
-    mx_grid(rows, K, mx_many_rows(src_dtype), vector, &grid, &block, &many);
     const int k = static_cast<int>(K);
     const long long r = rows, l = ld;
+    if (size == 2 && reinterpret_cast<uintptr_t>(src) % 32 == 0 && (rows == 1 || ld % 16 == 0)) {
+        mx_grid(rows, K, 16, 1, true, &grid, &block, &many);
+        const uint16_t* const s = static_cast<const uint16_t*>(src);
+        return src_dtype == FEATHER_SRC_BF16 ? mx_launch("mxfp4_quantize", mx_quantize16_kernel<FEATHER_SRC_BF16>, grid, block, stream, s, r, k, l, data, scales)
+                                             : mx_launch("mxfp4_quantize", mx_quantize16_kernel<FEATHER_SRC_FP16>, grid, block, stream, s, r, k, l, data, scales);
+    }
+    mx_grid(rows, K, 8, mx_many_rows(src_dtype), vector, &grid, &block, &many);
     switch (src_dtype) {
         case FEATHER_SRC_FP32: return mx_launch_quantize<FEATHER_SRC_FP32>(many, vector, grid, block, stream, src, r, k, l, data, scales);
         case FEATHER_SRC_BF16: return mx_launch_quantize<FEATHER_SRC_BF16>(many, vector, grid, block, stream, src, r, k, l, data, scales);
@@ -237,7 +293,7 @@ extern "C" int feather_mxfp4_dequantize(const uint8_t* data, const uint8_t* scal
     if (!mx_aligned16(data) || !mx_aligned16(scales) || !mx_aligned16(dst)) return set_error(FEATHER_ERR_BAD_ARGUMENT, "data, scales and dst must be 16-byte aligned");
     dim3 grid, block;
     bool many;
-    mx_grid(rows, K, mx_many_rows(dst_dtype), true, &grid, &block, &many);
+    mx_grid(rows, K, 8, mx_many_rows(dst_dtype), true, &grid, &block, &many);
     const int k = static_cast<int>(K);
     const long long r = rows;
     switch (dst_dtype) {

@@ -90,6 +90,32 @@ def test_quantise_strided_and_misaligned_rows(mx, cuda_dev, dtype):
         assert torch.equal(mx.unprepack_mxfp4_scales(scales, *view.shape), mx.unprepack_mxfp4_scales(ref_scales, *view.shape))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k", [(1030, 5120), (4111, 96), (2100, 1312)])
+def test_quantise_many_rows_of_every_alignment(mx, cuda_dev, rows, k, dtype):
+    """Rows that begin on 32-byte, 16-byte and element boundaries only, each of them pitched and not: the loads differ, the bits do not."""
+    x = _rows(rows, k, dtype, 5, cuda_dev)
+    codes, ref_scales = mx_ref.quantize(x)
+    packed = mx_ref.pack(codes)
+    for first, pitch in ((0, k), (8, k), (3, k), (0, k + 16), (0, k + 8), (16, k + 32), (8, k + 24), (1, k + 1)):
+        flat = torch.full((first + rows * pitch,), float("nan"), dtype=dtype, device=cuda_dev)
+        view = flat[first:].view(rows, pitch)[:, :k]
+        view.copy_(x)
+        data, scales = mx.quantize_mxfp4(view)
+        assert torch.equal(data, packed) and torch.equal(mx.unprepack_mxfp4_scales(scales, rows, k), ref_scales), (first, pitch)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_quantise_every_16_bit_value(mx, cuda_dev, dtype):
+    """All 65 536 patterns, among neighbours of their own size and among far smaller and larger ones."""
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16)
+    shuffled = bits[torch.randperm(65536, generator=torch.Generator().manual_seed(1))]
+    x = torch.cat([bits, shuffled]).view(dtype).view(-1, 64).to(cuda_dev)
+    data, scales = mx.quantize_mxfp4(x)
+    codes, ref = mx_ref.quantize(x)
+    assert torch.equal(mx.unprepack_mxfp4_scales(scales, len(x), 64), ref) and torch.equal(data, mx_ref.pack(codes))
+
+
 def test_empty_calls(mx, cuda_dev):
     data, scales = mx.quantize_mxfp4(torch.empty((0, 64), device=cuda_dev))
     assert data.shape == (0, 32) and scales.shape == (0, 1, 512)
