@@ -675,20 +675,23 @@ __global__ void __maxnreg__(DENSE ? 48 : 64) gated_norm_row_kernel(const __grid_
 }
 
 // ------------------------------------------------------------------------------------------------ single elements
-// Rows that are not 16-byte aligned or not a multiple of eight long: a block takes a row, a thread NE elements of it, `threads` apart.
+// Rows that are not 16-byte aligned or not a multiple of eight long: a block takes a row, a warp NE * 32 elements of it, a lane every 32nd of
+// those, so that a thread's addresses are one pointer and constants.  Element i exists if 32 i < left.
+// Bound by instructions (79 % of the issue slots where the row's threads took every blockDim-th element: 36 us for 4000 x 1027 fp16 with a
+// norm of y and a modulation, 21 us this way); a second copy of the code for warps whose part is whole, without the checks, takes 28 us.
 template <int NE>
-__device__ __forceinline__ void load_elements(uint32_t (&r)[NE], const void* base, int type, long long at, int step, int count) {
+__device__ __forceinline__ void load_elements(uint32_t (&r)[NE], const void* base, int type, long long at, int left) {
     if (base == nullptr) return;
     if (type == FEATHER_SRC_FP32) {
         const uint32_t* const q = static_cast<const uint32_t*>(base) + at;
 #pragma unroll
         for (int i = 0; i < NE; ++i)
-            if (i < count) r[i] = __ldg(q + i * step);
+            if (32 * i < left) r[i] = __ldg(q + 32 * i);
     } else {
         const uint16_t* const q = static_cast<const uint16_t*>(base) + at;
 #pragma unroll
         for (int i = 0; i < NE; ++i)
-            if (i < count) r[i] = __ldg(q + i * step);
+            if (32 * i < left) r[i] = __ldg(q + 32 * i);
     }
 }
 // The type is looked at once for a thread's elements, not for each.
@@ -706,23 +709,19 @@ __device__ __forceinline__ void each_element(const uint32_t (&r)[NE], int type, 
     }
 }
 template <int NE>
-__device__ __forceinline__ void store_elements(void* base, int type, long long at, int step, int count, const float (&v)[NE]) {
-    if (type == FEATHER_SRC_FP32) {
-        float* const o = static_cast<float*>(base) + at;
+__device__ __forceinline__ void store_elements(void* base, int type, long long at, int left, const float (&v)[NE]) {
+    const auto store = [&](auto* o, auto convert) {
 #pragma unroll
         for (int i = 0; i < NE; ++i)
-            if (i < count) o[i * step] = v[i];
-    } else {
-        uint16_t* const o = static_cast<uint16_t*>(base) + at;
-        const bool bf16 = type == FEATHER_SRC_BF16;
-#pragma unroll
-        for (int i = 0; i < NE; ++i)
-            if (i < count) o[i * step] = static_cast<uint16_t>(pack16x2(v[i], 0.0f, bf16));
-    }
+            if (32 * i < left) o[32 * i] = convert(v[i]);
+    };
+    if (type == FEATHER_SRC_FP32) store(static_cast<float*>(base) + at, [](float f) { return f; });
+    else if (type == FEATHER_SRC_BF16) store(static_cast<__nv_bfloat16*>(base) + at, [](float f) { return __float2bfloat16_rn(f); });
+    else store(static_cast<__half*>(base) + at, [](float f) { return __float2half_rn(f); });
 }
 
 template <int NE>
-__device__ __forceinline__ float normalise_elements(float (&v)[NE], const NormParams& p, int count, float (*part)[kNormMaxWarps], int& flip) {
+__device__ __forceinline__ float normalise_elements(float (&v)[NE], const NormParams& p, int left, float (*part)[kNormMaxWarps], int& flip) {
     if (p.a.kind == FEATHER_NORM_LAYER) {
         float s = 0.0f;
 #pragma unroll
@@ -730,7 +729,7 @@ __device__ __forceinline__ float normalise_elements(float (&v)[NE], const NormPa
         const float mean = row_sum<false>(s, part, flip) * p.inv_cols;
 #pragma unroll
         for (int i = 0; i < NE; ++i)
-            if (i < count) v[i] -= mean;
+            if (32 * i < left) v[i] -= mean;
     }
     float s = 0.0f;
 #pragma unroll
@@ -738,62 +737,61 @@ __device__ __forceinline__ float normalise_elements(float (&v)[NE], const NormPa
     return 1.0f / sqrtf(row_sum<false>(s, part, flip) * p.inv_cols + p.a.eps);
 }
 
-// EARLY: what makes r is loaded together, what makes h of it before the second norm's sums; otherwise each where it is used.
+// EARLY: what makes r is loaded together, what makes h of it before the second norm's sums; otherwise each where it is used.  48 registers there
+// (62 without the bound) let all of 999 rows of 1027 be resident at once: 7.9 us and 9.1 us with a modulation of each row, and 8.9 us with 40.
 template <int NE, bool EARLY>
-__global__ void __launch_bounds__(EARLY ? 512 : 1024) gated_norm_elements_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(EARLY ? 256 : 1024, EARLY ? 5 : 1) gated_norm_elements_kernel(const __grid_constant__ NormParams p) {
     __shared__ __align__(16) float part[2][kNormMaxWarps];
     const feather_norm_args& a = p.a;
     clear_parts(part);
     pdl_launch_dependents();
     pdl_wait_for_previous_kernel();
     const long long row = blockIdx.x;
-    const int t = threadIdx.x, step = blockDim.x;
-    const int count = p.vecs > t ? min(NE, (p.vecs - t + step - 1) / step) : 0;
+    const int at = (threadIdx.x >> 5) * (32 * NE) + (threadIdx.x & 31), left = p.vecs - at;
     int flip = 0;
     const ModulationAt m = modulation_at(a, row);
-    const long long gate_at = m.gate + t, scale_at = m.scale + t, shift_at = m.shift + t;
-    uint32_t x[NE], y[NE], gate[NE], post_weight[NE], weight[NE], bias[NE], scale[NE], shift[NE];
-    load_elements<NE>(x, a.x, a.x_dtype, row * a.ldx + t, step, count);
-    load_elements<NE>(y, a.y, a.y_dtype, row * a.ldy + t, step, count);
+    uint32_t x[NE] = {}, y[NE] = {}, gate[NE], post_weight[NE], weight[NE], bias[NE], scale[NE], shift[NE];
+    load_elements<NE>(x, a.x, a.x_dtype, row * a.ldx + at, left);
+    load_elements<NE>(y, a.y, a.y_dtype, row * a.ldy + at, left);
     const auto load_before = [&]() {
-        load_elements<NE>(gate, a.gate, a.gate_dtype, gate_at, step, count);
-        load_elements<NE>(post_weight, a.post_weight, a.post_weight_dtype, t, step, count);
+        load_elements<NE>(gate, a.gate, a.gate_dtype, m.gate + at, left);
+        load_elements<NE>(post_weight, a.post_weight, a.post_weight_dtype, at, left);
     };
     if (EARLY) load_before();
     float v[NE];                                                              // elements past the row are zero until the sums are done
     if (a.y != nullptr) {
-        each_element<NE>(y, a.y_dtype, [&](int i, float e) { v[i] = i < count ? e : 0.0f; });
-        const float inv = a.post_norm ? normalise_elements<NE>(v, p, count, part, flip) : 1.0f;
+        each_element<NE>(y, a.y_dtype, [&](int i, float e) { v[i] = e; });
+        const float inv = a.post_norm ? normalise_elements<NE>(v, p, left, part, flip) : 1.0f;
         if (!EARLY) load_before();
 #pragma unroll
         for (int i = 0; i < NE; ++i) v[i] *= inv * a.residual_scale;
         if (a.gate != nullptr) each_element<NE>(gate, a.gate_dtype, [&](int i, float e) { v[i] *= e; });
         if (a.post_weight != nullptr) each_element<NE>(post_weight, a.post_weight_dtype, [&](int i, float e) { v[i] *= e; });
-        each_element<NE>(x, a.x_dtype, [&](int i, float e) { v[i] = i < count ? v[i] + e : 0.0f; });
-        if (a.r != nullptr) store_elements<NE>(a.r, a.x_dtype, row * a.ldr + t, step, count, v);
+        each_element<NE>(x, a.x_dtype, [&](int i, float e) { v[i] = 32 * i < left ? v[i] + e : 0.0f; });
+        if (a.r != nullptr) store_elements<NE>(a.r, a.x_dtype, row * a.ldr + at, left, v);
     } else {
-        each_element<NE>(x, a.x_dtype, [&](int i, float e) { v[i] = i < count ? e : 0.0f; });
+        each_element<NE>(x, a.x_dtype, [&](int i, float e) { v[i] = e; });
     }
     if (a.h == nullptr) return;
     if (EARLY) {
-        load_elements<NE>(weight, a.weight, a.weight_dtype, t, step, count);
-        load_elements<NE>(bias, a.bias, a.bias_dtype, t, step, count);
-        load_elements<NE>(scale, a.scale, a.scale_dtype, scale_at, step, count);
-        load_elements<NE>(shift, a.shift, a.shift_dtype, shift_at, step, count);
+        load_elements<NE>(weight, a.weight, a.weight_dtype, at, left);
+        load_elements<NE>(bias, a.bias, a.bias_dtype, at, left);
+        load_elements<NE>(scale, a.scale, a.scale_dtype, m.scale + at, left);
+        load_elements<NE>(shift, a.shift, a.shift_dtype, m.shift + at, left);
     }
-    const float inv = normalise_elements<NE>(v, p, count, part, flip);
+    const float inv = normalise_elements<NE>(v, p, left, part, flip);
 #pragma unroll
     for (int i = 0; i < NE; ++i) v[i] *= inv;
-    const auto apply = [&](uint32_t(&r)[NE], const void* base, int type, long long at, auto op) {
+    const auto apply = [&](uint32_t(&r)[NE], const void* base, int type, long long from, auto op) {
         if (base == nullptr) return;
-        if (!EARLY) load_elements<NE>(r, base, type, at, step, count);
+        if (!EARLY) load_elements<NE>(r, base, type, from, left);
         each_element<NE>(r, type, op);
     };
-    apply(weight, a.weight, a.weight_dtype, t, [&](int i, float e) { v[i] *= e; });
-    apply(bias, a.bias, a.bias_dtype, t, [&](int i, float e) { v[i] += e; });
-    apply(scale, a.scale, a.scale_dtype, scale_at, [&](int i, float e) { v[i] *= 1.0f + e; });
-    apply(shift, a.shift, a.shift_dtype, shift_at, [&](int i, float e) { v[i] += e; });
-    store_elements<NE>(a.h, a.h_dtype, row * a.ldh + t, step, count, v);
+    apply(weight, a.weight, a.weight_dtype, at, [&](int i, float e) { v[i] *= e; });
+    apply(bias, a.bias, a.bias_dtype, at, [&](int i, float e) { v[i] += e; });
+    apply(scale, a.scale, a.scale_dtype, m.scale + at, [&](int i, float e) { v[i] *= 1.0f + e; });
+    apply(shift, a.shift, a.shift_dtype, m.shift + at, [&](int i, float e) { v[i] += e; });
+    store_elements<NE>(a.h, a.h_dtype, row * a.ldh + at, left, v);
 }
 
 // ------------------------------------------------------------------------------------------------ launches
@@ -997,7 +995,7 @@ extern "C" int feather_gated_norm(const feather_norm_args* args_host, feather_st
     cudaError_t e;
     const auto threads = [&](int n) { return (p.vecs + 32 * n - 1) / (32 * n) * 32; };
     if (vector) e = norm_launch(p, sms, stream);
-    else if (p.vecs <= 2048) e = norm_launch_kernel(gated_norm_elements_kernel<4, true>, a.rows, threads(4), 0, stream, p);
+    else if (p.vecs <= 2048) e = norm_launch_kernel(gated_norm_elements_kernel<8, true>, a.rows, threads(8), 0, stream, p);
     else e = norm_launch_kernel(gated_norm_elements_kernel<16, false>, a.rows, threads(16), 0, stream, p);
     if (e != cudaSuccess) return set_error(FEATHER_ERR_CUDA, "gated_norm launch failed: %s", cudaGetErrorString(e));
     return FEATHER_OK;

@@ -105,6 +105,20 @@ def test_thousands_of_rows_without_a_norm_of_y(norm, cuda_dev, x_dtype, y_dtype)
         _check(norm, x, None, bias=_t((cols,), 8, cuda_dev), kind="layer")
 
 
+@pytest.mark.parametrize("cols", [1, 2, 31, 33, 255, 257, 513, 1027, 2047, 2049, 4099, 8191, 15873, 16383])
+def test_odd_widths_beside_a_warp_and_a_block(norm, cuda_dev, cols):
+    """Widths where a warp's part of a row is one element, whole, or short of whole by one, in rows that begin at every alignment; r alone and
+    h alone."""
+    x, y = _t((2, 5, cols), 1, cuda_dev, FP16, about=0.5), _t((2, 5, cols), 2, cuda_dev, BF16)
+    for kind in ("rms", "layer"):
+        r, h = _check(norm, x, y, gate=_t((2, 5, cols), 3, cuda_dev), post_norm=True, post_weight=_t((cols,), 6, cuda_dev, BF16, 0.2, 1.0),
+                      scale=_t((2, 1, cols), 4, cuda_dev, FP16, 0.2), shift=_t((cols,), 5, cuda_dev, BF16), kind=kind)
+        _check(norm, x, None, kind=kind, weight=_t((cols,), 7, cuda_dev, FP16, 0.2, 1.0), bias=_t((cols,), 8, cuda_dev))
+    alone, none = norm.gated_residual_norm(x, y, gate=_t((cols,), 9, cuda_dev), want_norm=False)
+    both, _ = norm.gated_residual_norm(x, y, gate=_t((cols,), 9, cuda_dev))
+    assert none is None and torch.equal(alone, both)
+
+
 @pytest.mark.parametrize("x_dtype", [BF16, FP16, FP32])
 @pytest.mark.parametrize("y_dtype", [BF16, FP16, FP32])
 def test_types(norm, cuda_dev, x_dtype, y_dtype):
