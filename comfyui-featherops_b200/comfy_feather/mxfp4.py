@@ -65,6 +65,12 @@ class FeatherMXFP4Layout(QuantizedLayout):
         return {"": qdata, "_scale": mxfp4.unprepack_mxfp4_scales(params.scale, n, k)}
 
 
+def scaled_weight(weight, scale):
+    """The values of a scaled checkpoint weight, in fp32."""
+    weight = weight.to(torch.float32)
+    return weight if scale is None else weight * scale.to(device=weight.device, dtype=torch.float32)
+
+
 def make_mxfp4_weight(weight, scale, orig_dtype):
     """The weight of a checkpoint as an MXFP4 `QuantizedTensor` that reads as `orig_dtype`."""
     if weight.ndim != 2:
@@ -76,9 +82,7 @@ def make_mxfp4_weight(weight, scale, orig_dtype):
         params = FeatherMXFP4Params(scale=mxfp4.prepack_mxfp4_scales(scale.to(weight.device)), orig_dtype=orig_dtype, orig_shape=(n, k))
         return QuantizedTensor(weight.contiguous(), FEATHER_MXFP4_LAYOUT, params)
     if scale is not None or weight.dtype not in _SOURCES:
-        weight = weight.to(torch.float32)
-        if scale is not None:
-            weight = weight * scale.to(device=weight.device, dtype=torch.float32)
+        weight = scaled_weight(weight, scale)
     data, scales = _quantize(weight)
     return QuantizedTensor(data, FEATHER_MXFP4_LAYOUT, FeatherMXFP4Params(scale=scales, orig_dtype=orig_dtype, orig_shape=tuple(weight.shape)))
 

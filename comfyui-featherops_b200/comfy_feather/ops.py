@@ -21,7 +21,7 @@ from ..kernel.convert import bf16_to_fp16
 from ..kernel.hip.hip_kernel import scaled_mm_b200, scaled_mm_lora
 from ..kernel.mxfp4 import linear_mxfp4
 from .lora import apply_lora_patches, fused_lora_operands
-from .mxfp4 import get_mxfp4_plain_tensors, is_mxfp4_weight, make_mxfp4_weight, quantize_mxfp4_weight
+from .mxfp4 import get_mxfp4_plain_tensors, is_mxfp4_weight, make_mxfp4_weight, quantize_mxfp4_weight, scaled_weight
 from .quant import get_feather_plain_tensors, is_feather_quantized_weight, make_feather_quantized_weight, quantize_feather_weight
 
 
@@ -138,7 +138,8 @@ class _FeatherLinear:
 
 
 class _FeatherMXFP4Linear(_FeatherLinear):
-    """The same Linear with an MXFP4 weight.  Un-merged LoRA patches are added after the product."""
+    """The same Linear with an MXFP4 weight.  Un-merged LoRA patches are added after the product.  A layer that stays plain takes the
+    checkpoint's scale into its weight (with K % 32 == 16 that is one which the fp8 format would have quantised)."""
 
     def _keeps_plain_weight(self, prefix, weight):
         return super()._keeps_plain_weight(prefix, weight) or self.in_features % 32 != 0
@@ -154,8 +155,11 @@ class _FeatherMXFP4Linear(_FeatherLinear):
                 weight = make_mxfp4_weight(weight, scale, self.out_dtype)
             elif weight.dtype == torch.uint8:                      # MXFP4 in the checkpoint, excluded here
                 weight = make_mxfp4_weight(weight, scale, self.out_dtype).dequantize()
-            elif self.in_features % 32 != 0:
-                print(f"Warning: Not MXFP4 {prefix}weight {tuple(weight.shape)}")
+            else:
+                if self.in_features % 32 != 0:
+                    print(f"Warning: Not MXFP4 {prefix}weight {tuple(weight.shape)}")
+                if scale is not None:
+                    weight = scaled_weight(weight, scale).to(self.out_dtype)
             self.weight = _frozen(weight)
         self.bias = None if bias is None else _frozen(bias.to(self.out_dtype))
 

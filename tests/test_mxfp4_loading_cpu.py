@@ -1,0 +1,40 @@
+"""CPU: what the MXFP4 Linear makes of a checkpoint's weight and scale where no kernel is needed."""
+
+import importlib
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+FP8 = (torch.float8_e5m2, torch.float8_e4m3fn)
+
+
+@pytest.fixture(scope="module")
+def ops_mod(pkg):
+    return importlib.import_module("feather_b200.comfy_feather.ops")
+
+
+def _linear(ops_mod, k, n, state, excluded=(), out_dtype=torch.bfloat16):
+    lin = ops_mod.feather_ops(out_dtype=out_dtype, excluded_names=excluded, weight_format="mxfp4").Linear(k, n, bias=False)
+    lin._load_from_state_dict({"blocks.0.ffn." + key: v for key, v in state.items()}, "blocks.0.ffn.", {}, True, [], [], [])
+    return lin
+
+
+@pytest.mark.parametrize("key", ["weight_scale", "scale_weight"])
+@pytest.mark.parametrize("dtype", FP8)
+@pytest.mark.parametrize("k,excluded", [(48, ()), (16, ()), (64, ("ffn",)), (72, ())])
+def test_a_plain_layer_keeps_its_scale(ops_mod, k, excluded, dtype, key):
+    """Layers that stay un-quantised (K not a multiple of 32, or excluded by name) hold the values the checkpoint stands for."""
+    g = torch.Generator().manual_seed(k)
+    codes, scale = torch.randn((40, k), generator=g).to(dtype), torch.tensor(0.3)
+    lin = _linear(ops_mod, k, 40, {"weight": codes, key: scale}, excluded)
+    want = (codes.float() * scale).to(torch.bfloat16)
+    assert not lin.is_quantized and lin.weight.dtype == torch.bfloat16 and torch.equal(lin.weight, want)
+    x = torch.randn((3, k), generator=g)
+    assert torch.equal(lin(x), F.linear(x, want.float()))
+
+
+def test_a_plain_layer_without_a_scale_is_left_alone(ops_mod):
+    for weight in (torch.randn(40, 48), torch.randn(40, 48).to(torch.float8_e5m2)):
+        lin = _linear(ops_mod, 48, 40, {"weight": weight})
+        assert lin.weight.dtype == weight.dtype and torch.equal(lin.weight.float(), weight.float())
