@@ -1,5 +1,8 @@
 // MXFP4 weight and activation format: quantise rows of fp32 / bf16 / fp16 and the inverse.  The format is in mxfp4.cuh.
 //
+// All loads are ordinary ones, without __ldg or __restrict__: a kernel may be resident while the one before it still writes its source, and
+// the read-only path asks for memory that nobody writes during the kernel's life.
+//
 // Both are byte movers.  A lane holds eight elements, four lanes a block of 32 (16 and two for aligned 16-bit sources), so the block's
 // maximum is a shuffle or two and all loads and stores are whole vectors; nothing is staged and every byte is touched once.
 #include <cuda_runtime.h>
@@ -30,16 +33,16 @@ __device__ __forceinline__ void mx_load8(const void* p, MxRaw<kSrc>& r) {
     if constexpr (kVector) {
 #pragma unroll
         for (int i = 0; i < kWords / 4; ++i) {
-            const uint4 a = __ldg(static_cast<const uint4*>(p) + i);
+            const uint4 a = static_cast<const uint4*>(p)[i];
             r.w[4 * i] = a.x; r.w[4 * i + 1] = a.y; r.w[4 * i + 2] = a.z; r.w[4 * i + 3] = a.w;
         }
     } else if constexpr (kSrc == FEATHER_SRC_FP32) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) r.w[i] = __ldg(static_cast<const uint32_t*>(p) + i);
+        for (int i = 0; i < 8; ++i) r.w[i] = static_cast<const uint32_t*>(p)[i];
     } else {
         const uint16_t* const h = static_cast<const uint16_t*>(p);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r.w[i] = static_cast<uint32_t>(__ldg(h + 2 * i)) | (static_cast<uint32_t>(__ldg(h + 2 * i + 1)) << 16);
+        for (int i = 0; i < 4; ++i) r.w[i] = static_cast<uint32_t>(h[2 * i]) | (static_cast<uint32_t>(h[2 * i + 1]) << 16);
     }
 }
 template <int kSrc>
@@ -85,7 +88,7 @@ __device__ __forceinline__ uint32_t mx_block_top(const MxRaw<kSrc>& r) {
 // kRows rows, ty apart, and has all their loads under way at once.
 template <int kSrc, int kRows, bool kVector>
 __global__ void __launch_bounds__(kMxThreads)
-mx_quantize_kernel(const void* __restrict__ src, long long rows, int k, long long ld, uint8_t* __restrict__ data, uint8_t* __restrict__ scales) {
+mx_quantize_kernel(const void* src, long long rows, int k, long long ld, uint8_t* data, uint8_t* scales) {
     constexpr int kSize = kSrc == FEATHER_SRC_FP32 ? 4 : 2;
     pdl_launch_dependents();
     pdl_wait_for_previous_kernel();
@@ -119,7 +122,7 @@ mx_quantize_kernel(const void* __restrict__ src, long long rows, int k, long lon
 // lane, 1024 x 5120 3.9 and 4.9 us.  tx is a multiple of 8 (four blocks sit in a quarter-warp); src and its rows are 32-byte aligned.
 template <int kSrc>
 __global__ void __launch_bounds__(kMxThreads)
-mx_quantize16_kernel(const uint16_t* __restrict__ src, long long rows, int k, long long ld, uint8_t* __restrict__ data, uint8_t* __restrict__ scales) {
+mx_quantize16_kernel(const uint16_t* src, long long rows, int k, long long ld, uint8_t* data, uint8_t* scales) {
     pdl_launch_dependents();
     pdl_wait_for_previous_kernel();
     const long long row = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y;
@@ -129,9 +132,10 @@ mx_quantize16_kernel(const uint16_t* __restrict__ src, long long rows, int k, lo
     const uint16_t* const from = src + row * ld + vec * 16;
     uint32_t raw[8] = {};
     if (in && row < rows)
-        asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                      : "=r"(raw[0]), "=r"(raw[1]), "=r"(raw[2]), "=r"(raw[3]), "=r"(raw[4]), "=r"(raw[5]), "=r"(raw[6]), "=r"(raw[7])
-                     : "l"(from));
+                     : "l"(from)
+                     : "memory");
     uint2* const to = reinterpret_cast<uint2*>(data) + row * (k / 16) + vec;
     uint32_t top = 0;
 #pragma unroll
@@ -157,7 +161,7 @@ mx_quantize16_kernel(const uint16_t* __restrict__ src, long long rows, int k, lo
 
 template <int kDst, int kRows>
 __global__ void __launch_bounds__(kMxThreads)
-mx_dequantize_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict__ scales, long long rows, int k, void* __restrict__ dst) {
+mx_dequantize_kernel(const uint8_t* data, const uint8_t* scales, long long rows, int k, void* dst) {
     pdl_launch_dependents();
     pdl_wait_for_previous_kernel();
     const long long row0 = static_cast<long long>(blockIdx.x) * (blockDim.y * kRows) + threadIdx.y;
@@ -169,8 +173,8 @@ mx_dequantize_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict
     for (int r = 0; r < kRows; ++r) {
         const long long row = row0 + r * blockDim.y;
         if (row < rows) {
-            q[r] = __ldg(reinterpret_cast<const uint32_t*>(data) + row * (k / 8) + vec);
-            code[r] = __ldg(scales + mx_scale_word_offset(row, block >> 2, mx_tiles_k(k)) + (block & 3));
+            q[r] = reinterpret_cast<const uint32_t*>(data)[row * (k / 8) + vec];
+            code[r] = scales[mx_scale_word_offset(row, block >> 2, mx_tiles_k(k)) + (block & 3)];
         }
     }
 #pragma unroll

@@ -130,7 +130,7 @@ struct MxMmParams {
 };
 
 __device__ __forceinline__ float load16(const uint16_t* p, bool bf16) {
-    const uint16_t v = __ldg(p);
+    const uint16_t v = *p;                              // not __ldg: the kernel before this one may have written it
     return bf16 ? __uint_as_float(static_cast<uint32_t>(v) << 16) : __half2float(__ushort_as_half(v));
 }
 __device__ __forceinline__ uint16_t round16(float v, bool bf16) { return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v)); }

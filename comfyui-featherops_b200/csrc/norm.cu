@@ -53,6 +53,9 @@ __device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
 }
 
 // ------------------------------------------------------------------------------------------------ memory <-> registers
+// Every load here is an ordinary one: the kernels may be resident while the kernel before them still writes their operands, so the
+// read-only path (__ldg), which asks for memory that nobody writes during the kernel's life, is not theirs to take.
+//
 // Eight consecutive elements as they lie in memory (16-byte aligned).
 template <int T>
 struct alignas(16) Raw8 {
@@ -63,11 +66,11 @@ __device__ __forceinline__ Raw8<T> load8(const void* base, long long at) {
     Raw8<T> r;
     if constexpr (T == FEATHER_SRC_FP32) {
         const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(base) + at);
-        const uint4 a = __ldg(p), b = __ldg(p + 1);
+        const uint4 a = p[0], b = p[1];
         r.w[0] = a.x; r.w[1] = a.y; r.w[2] = a.z; r.w[3] = a.w;
         r.w[4] = b.x; r.w[5] = b.y; r.w[6] = b.z; r.w[7] = b.w;
     } else {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at));
+        const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at);
         r.w[0] = a.x; r.w[1] = a.y; r.w[2] = a.z; r.w[3] = a.w;
     }
     return r;
@@ -686,12 +689,12 @@ __device__ __forceinline__ void load_elements(uint32_t (&r)[NE], const void* bas
         const uint32_t* const q = static_cast<const uint32_t*>(base) + at;
 #pragma unroll
         for (int i = 0; i < NE; ++i)
-            if (32 * i < left) r[i] = __ldg(q + 32 * i);
+            if (32 * i < left) r[i] = q[32 * i];
     } else {
         const uint16_t* const q = static_cast<const uint16_t*>(base) + at;
 #pragma unroll
         for (int i = 0; i < NE; ++i)
-            if (32 * i < left) r[i] = __ldg(q + 32 * i);
+            if (32 * i < left) r[i] = q[32 * i];
     }
 }
 // The type is looked at once for a thread's elements, not for each.
