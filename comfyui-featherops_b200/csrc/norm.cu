@@ -10,6 +10,7 @@
 // product that follows (mxfp4.cuh).
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <stdlib.h>
 
 #include <mutex>
 #include <type_traits>
@@ -132,6 +133,7 @@ struct NormParams {
     int chunk;            // consecutive rows of a warp or block
     int groups, stages;   // of the kernel for many rows
     float inv_cols;
+    uint64_t wait_ns;     // limit of its waits for a row
 };
 
 // ------------------------------------------------------------------------------------------------ sums over a row
@@ -447,48 +449,45 @@ __global__ void __maxnreg__(norm_regs(NV, POST)) gated_norm_groups_kernel(const 
     };
     if (t == 0)
         for (int s = 0; s < p.stages; ++s) fetch();
-    long long change = begin;
+    const auto fold = [&](long long first) {                                  // the coefficients of the rows from `first` on, by the whole block
+        __syncthreads();                                                      // nobody reads the old ones any more
+        const ModulationAt m = modulation_at(a, first);
+        for (int vec = threadIdx.x; vec < p.vecs; vec += blockDim.x) {
+            RawAny q, w;
+            float f[8], h[8];
+            if (present & kNormG) {
+                load_any(q, a.gate, a.gate_dtype, m.gate + vec * 8);
+                load_any(w, a.post_weight, a.post_weight_dtype, vec * 8);
+                fold_g(a, q, w, f);
+                dynamic[vec] = make_float4(f[0], f[1], f[2], f[3]);
+                dynamic[p.vecs + vec] = make_float4(f[4], f[5], f[6], f[7]);
+            }
+            if (present & (kNormA | kNormB)) {
+                load_any(q, a.scale, a.scale_dtype, m.scale + vec * 8);
+                load_any(w, a.bias, a.bias_dtype, vec * 8);
+                start_ab(a, q, w, f, h);
+                load_any(q, a.weight, a.weight_dtype, vec * 8);
+                load_any(w, a.shift, a.shift_dtype, m.shift + vec * 8);
+                finish_ab(a, q, w, f, h);
+                dynamic[kept_step + vec] = make_float4(f[0], f[1], f[2], f[3]);
+                dynamic[kept_step + p.vecs + vec] = make_float4(f[4], f[5], f[6], f[7]);
+                dynamic[2 * kept_step + vec] = make_float4(h[0], h[1], h[2], h[3]);
+                dynamic[2 * kept_step + p.vecs + vec] = make_float4(h[4], h[5], h[6], h[7]);
+            }
+        }
+        __syncthreads();
+    };
+    long long wave = begin, change = begin;
     int slot = 0;
     uint32_t parity = 0;
-    for (long long wave = begin; wave < end; wave = min(wave + p.groups, change)) {
+    for (; wave < end; wave = min(wave + p.groups, change)) {
         if (wave >= change) {
             change = KEEP ? min(end, next_change(a, wave)) : end;
-            if (KEEP && present != 0) {
-                __syncthreads();                                              // nobody reads the old ones any more
-                const ModulationAt m = modulation_at(a, wave);
-                for (int vec = threadIdx.x; vec < p.vecs; vec += blockDim.x) {
-                    RawAny q, w;
-                    float f[8], h[8];
-                    if (present & kNormG) {
-                        load_any(q, a.gate, a.gate_dtype, m.gate + vec * 8);
-                        load_any(w, a.post_weight, a.post_weight_dtype, vec * 8);
-                        fold_g(a, q, w, f);
-                        dynamic[vec] = make_float4(f[0], f[1], f[2], f[3]);
-                        dynamic[p.vecs + vec] = make_float4(f[4], f[5], f[6], f[7]);
-                    }
-                    if (present & (kNormA | kNormB)) {
-                        load_any(q, a.scale, a.scale_dtype, m.scale + vec * 8);
-                        load_any(w, a.bias, a.bias_dtype, vec * 8);
-                        start_ab(a, q, w, f, h);
-                        load_any(q, a.weight, a.weight_dtype, vec * 8);
-                        load_any(w, a.shift, a.shift_dtype, m.shift + vec * 8);
-                        finish_ab(a, q, w, f, h);
-                        dynamic[kept_step + vec] = make_float4(f[0], f[1], f[2], f[3]);
-                        dynamic[kept_step + p.vecs + vec] = make_float4(f[4], f[5], f[6], f[7]);
-                        dynamic[2 * kept_step + vec] = make_float4(h[0], h[1], h[2], h[3]);
-                        dynamic[2 * kept_step + p.vecs + vec] = make_float4(h[4], h[5], h[6], h[7]);
-                    }
-                }
-                __syncthreads();
-            }
+            if (KEEP && present != 0) fold(wave);
         }
         const long long row = wave + group;
         if (row >= change) continue;                                          // a whole group
-        if (!mbar_wait(bar0 + 8 * slot, parity, &abort_flag)) {
-            // record it and go on: the barriers stay matched
-            abort_flag = 1;
-            if (a.status_dev != nullptr) atomicCAS(a.status_dev, 0, FEATHER_ERR_DEVICE_TIMEOUT | (1 << 8));
-        }
+        if (!__all_sync(0xffffffffu, mbar_wait_within(bar0 + 8 * slot, parity, &abort_flag, p.wait_ns))) break;     // the warp is lost
         const uint8_t* const from = ring + slot * row_bytes;
         if (++slot == p.stages) {
             slot = 0;
@@ -606,6 +605,43 @@ __global__ void __maxnreg__(norm_regs(NV, POST)) gated_norm_groups_kernel(const 
             store_all(std::integral_constant<int, FEATHER_SRC_FP16>{});
         } else {
             store_all(std::integral_constant<int, FEATHER_SRC_FP32>{});
+        }
+    }
+    if (wave >= end) return;
+    // A warp whose wait ran out reads and stores nothing from there on and keeps to the barriers; its part of a sum is NaN, and so is every h
+    // that would be made of it. The warp that fetches starts no further copy (its group's other warps are lost where a row was never fetched)
+    // and lets those in flight land, before the block gives its memory back.
+    abort_flag = 1;
+    if (a.status_dev != nullptr) atomicCAS(a.status_dev, 0, FEATHER_ERR_DEVICE_TIMEOUT | (1 << 8));
+    if (t == 0) {
+        const uint64_t begin_ns = globaltimer_ns();
+        long long until = change;
+        for (long long w = wave; w < fetch_wave; w = min(w + p.groups, until)) {             // as `fetch` went
+            if (w >= until) until = KEEP ? min(end, next_change(a, w)) : end;
+            if (w + group >= until) continue;
+            while (!mbar_try_wait(bar0 + 8 * slot, parity) && globaltimer_ns() - begin_ns < kWaitLimitNs) {
+            }
+            if (++slot == p.stages) {
+                slot = 0;
+                parity ^= 1u;
+            }
+        }
+    }
+    __syncwarp();
+    const int rounds = 1 + (sums.warps > 1 ? (POST && has_y && a.post_norm ? 1 : 0) + (a.h != nullptr ? 1 : 0) : 0);      // barriers of a row
+#pragma unroll 1
+    for (; wave < end; wave = min(wave + p.groups, change)) {
+        if (wave >= change) {
+            change = KEEP ? min(end, next_change(a, wave)) : end;
+            if (KEEP && present != 0) fold(wave);
+        }
+        if (wave + group >= change) continue;
+        barrier.sync();
+#pragma unroll 1
+        for (int i = 1; i < rounds; ++i) {
+            if ((threadIdx.x & 31) == 0) sums.part[sums.flip * kNormMaxWarps + sums.warp] = make_float2(__int_as_float(0x7FC00000), __int_as_float(0x7FC00000));
+            sums.flip ^= 1;
+            barrier.sync();
         }
     }
 }
@@ -808,6 +844,17 @@ static int norm_sm_count() {
     return cached[dev];
 }
 
+// Limit of a wait for a row of the ring: two seconds, or what FEATHER_NORM_WAIT_NS says if that is less (0: a row that is not there at the
+// first look counts as lost, which is how giving up is tested).
+static uint64_t norm_wait_ns() {
+    static const uint64_t ns = [] {
+        const char* const text = getenv("FEATHER_NORM_WAIT_NS");
+        const unsigned long long asked = text != nullptr ? strtoull(text, nullptr, 10) : kWaitLimitNs;
+        return asked < kWaitLimitNs ? static_cast<uint64_t>(asked) : kWaitLimitNs;
+    }();
+    return ns;
+}
+
 constexpr int kNormMaxSmem = 225 * 1024;      // dynamic, beside the sums and barriers
 
 template <typename... Params, typename... Args>
@@ -992,6 +1039,7 @@ extern "C" int feather_gated_norm(const feather_norm_args* args_host, feather_st
         a.ldh = a.cols / 8;                                                    // 32-bit words of a packed row
     }
     p.inv_cols = 1.0f / static_cast<float>(a.cols);
+    p.wait_ns = norm_wait_ns();
     p.vecs = static_cast<int>(vector ? a.cols / 8 : a.cols);
     const int sms = norm_sm_count();
     if (sms < 1) return set_error(FEATHER_ERR_CUDA, "the number of SMs could not be read");
