@@ -200,30 +200,40 @@ void check_product(const at::Device& device, int64_t k, const Packed& b, const a
     }
 }
 
-int launch_product(const uint8_t* a, const uint8_t* a_scales, const Packed& b, const at::Tensor* bias, const at::Tensor& out, int64_t m, int* status_dev, cudaStream_t stream) {
-    return g_lib.mm(a, a_scales, b.data.data_ptr<uint8_t>(), b.scales.data_ptr<uint8_t>(), bias != nullptr ? bias->data_ptr() : nullptr, out.data_ptr(), m, b.rows, b.k, b.rows,
+int launch_product(const uint8_t* a, const uint8_t* a_scales, const Packed& b, const at::Tensor* bias, const at::Tensor& out, int64_t m, int64_t ldc, int* status_dev, cudaStream_t stream) {
+    return g_lib.mm(a, a_scales, b.data.data_ptr<uint8_t>(), b.scales.data_ptr<uint8_t>(), bias != nullptr ? bias->data_ptr() : nullptr, out.data_ptr(), m, b.rows, b.k, ldc,
                     out.scalar_type() == at::kBFloat16 ? FEATHER_OUT_BF16 : FEATHER_OUT_FP16, status_dev, stream);
 }
 
 PyObject* py_mm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    TORCH_CHECK(n == 6, "mm(a, a_scales, b, b_scales, bias, out_dtype)");
+    TORCH_CHECK(n == 6 || n == 7, "mm(a, a_scales, b, b_scales, bias, out_dtype[, out])");
     const at::Tensor* const bias = optional_tensor(args[4], "bias");
     const auto out_dtype = optional_dtype(args[5], "out_dtype");
-    refuse_grad({bias}, "MXFP4 operators have");
+    const at::Tensor* const given = n == 7 ? optional_tensor(args[6], "out") : nullptr;
+    refuse_grad({bias, given}, "MXFP4 operators have");
     TORCH_CHECK(out_dtype && (*out_dtype == at::kHalf || *out_dtype == at::kBFloat16), "out_dtype must be float16 or bfloat16");
     const Packed a = packed(tensor(args[0], "a"), tensor(args[1], "a_scales"), "a"), b = packed(tensor(args[2], "b"), tensor(args[3], "b_scales"), "b");
     const at::Device device = a.data.device();
     check_product(device, a.k, b, bias, out_dtype);
+    int64_t ldc = b.rows;
+    if (given != nullptr) {
+        TORCH_CHECK(given->device() == device, "out must be on the same device as a");
+        TORCH_CHECK(given->scalar_type() == *out_dtype, "out must have the out dtype");
+        TORCH_CHECK(given->dim() == 2 && given->size(0) == a.rows && given->size(1) == b.rows, "out must be [", a.rows, ", ", b.rows, "], got ", given->sizes());
+        TORCH_CHECK(b.rows == 1 || given->stride(1) == 1, "out must have contiguous columns");
+        TORCH_CHECK(a.rows <= 1 || given->stride(0) >= b.rows, "rows of out overlap");
+        if (a.rows > 1) ldc = given->stride(0);
+    }
     int* const status_dev = status_word(device.index());
     at::Tensor out;
     int status = FEATHER_OK;
     {
         WithoutGil released;
         const c10::cuda::CUDAGuard guard(device);
-        out = empty({a.rows, b.rows}, *out_dtype, device);
+        out = given != nullptr ? *given : empty({a.rows, b.rows}, *out_dtype, device);
         if (a.rows != 0)
-            status = launch_product(a.data.data_ptr<uint8_t>(), a.scales.data_ptr<uint8_t>(), b, bias, out, a.rows, status_dev, c10::cuda::getCurrentCUDAStream(device.index()).stream());
+            status = launch_product(a.data.data_ptr<uint8_t>(), a.scales.data_ptr<uint8_t>(), b, bias, out, a.rows, ldc, status_dev, c10::cuda::getCurrentCUDAStream(device.index()).stream());
     }
     check(status, "feather_mxfp4_mm");
     return THPVariable_Wrap(std::move(out));
@@ -264,7 +274,7 @@ PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
             const Rows src = rows_of(x, k);
             const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
             quantised = g_lib.quantize(src.ptr, source_code(x.scalar_type()), m, k, src.ld, scales + scale_bytes, scales, stream);
-            if (quantised == FEATHER_OK) status = launch_product(scales + scale_bytes, scales, b, bias, out, m, status_dev, stream);
+            if (quantised == FEATHER_OK) status = launch_product(scales + scale_bytes, scales, b, bias, out, m, b.rows, status_dev, stream);
         }
     }
     check(quantised, "feather_mxfp4_quantize");

@@ -681,16 +681,5 @@ def binding():
 
 
 def mxfp4_mm_into(a, a_scales, b, b_scales, bias, c):
-    """c[:, :N] = round(a @ b^T + bias) with MXFP4 a [M, K/2] and b [N, K/2]; c may be a column slice of a wider row-major buffer."""
-    lib = load_library()
-    dev = _require_cuda(a, a_scales, b, b_scales, bias, c)
-    index = dev.index
-    st = status_word_for(dev)
-    with _OnDevice(index):
-        status = lib.feather_mxfp4_mm(
-            a.data_ptr(), a_scales.data_ptr(), b.data_ptr(), b_scales.data_ptr(), _addr(bias), c.data_ptr(), a.shape[0], b.shape[0], a.shape[1] * 2, c.stride(0),
-            _OUT_CODE[c.dtype], st.data_ptr(), _raw_stream(index),
-        )
-    if status != FEATHER_OK:
-        _check(status, "feather_mxfp4_mm")
-    return c
+    """c = round(a @ b^T + bias) with MXFP4 a [M, K/2] and b [N, K/2]; c [M, N] may be a column slice of a wider row-major buffer."""
+    return binding().mm(a, a_scales, b, b_scales, bias, c.dtype, c)

@@ -1,0 +1,52 @@
+"""CPU: further refusals of the MXFP4 operators and of the fused norm.  As in test_mxfp4_cpu.py, calls that would reach the GPU are made with fake
+CUDA tensors: the checks come before the first pointer."""
+
+import importlib
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+BF16 = torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def mx(pkg):
+    return importlib.import_module("feather_b200.kernel.mxfp4")
+
+
+@pytest.fixture(scope="module")
+def norm(pkg):
+    return importlib.import_module("feather_b200.kernel.norm")
+
+
+def test_product_into_a_given_output(native):
+    with FakeTensorMode():
+        def u8(*shape, device="cuda"):
+            return torch.empty(shape, dtype=torch.uint8, device=device)
+
+        def out(*shape, dtype=BF16, device="cuda"):
+            return torch.empty(shape, dtype=dtype, device=device)
+
+        a, sa, b, sb, bias = u8(4, 64), u8(1, 1, 512), u8(200, 64), u8(2, 1, 512), out(200)
+        for args, match in (
+            ((a, sa, b, sb, None, out(3, 200)), r"out must be \[4, 200\]"),                      # too few rows: would be written past its end
+            ((a, sa, b, sb, None, out(4, 199)), r"out must be \[4, 200\]"),
+            ((a, sa, b, sb, None, out(4 * 200)), r"out must be \[4, 200\]"),
+            ((a, sa, b, sb, None, out(200, 4).t()), "contiguous columns"),
+            ((a, sa, b, sb, None, out(1, 200).expand(4, 200)), "rows of out overlap"),
+            ((a, sa, b, sb, None, out(4, 200, device="cuda:1")), "same device"),
+            ((a, sa, b, sb, None, out(4, 200, device="cpu")), "same device"),
+            ((a, sa, b, sb, None, out(4, 200, dtype=torch.float32)), "out_dtype must be"),
+            ((a, sa, b, sb, bias, out(4, 200, dtype=torch.float16)), "bias must have the out dtype"),
+            ((a, sa, b, sb, bias[:7], out(4, 200)), "N elements"),
+            ((a, sa, u8(200, 96), u8(2, 2, 512), None, out(4, 200)), "same K"),
+            ((a, sa, b, sa, None, out(4, 200)), "b_scales must be"),
+            ((a, u8(1, 4, 128), b, sb, None, out(4, 200)), "a_scales must be"),
+            ((u8(64, 4).t(), sa, b, sb, None, out(4, 200)), "contiguous"),
+            ((a.float(), sa, b, sb, None, out(4, 200)), "uint8"),
+        ):
+            with pytest.raises(RuntimeError, match=match):
+                native.mxfp4_mm_into(*args)
+        with pytest.raises(RuntimeError, match="no backward"):
+            native.mxfp4_mm_into(a, sa, b, sb, None, out(4, 200).requires_grad_())
