@@ -62,6 +62,8 @@ int source_code(at::ScalarType t) {
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 void refuse_grad(std::initializer_list<const at::Tensor*> tensors, const char* what) {
+    for (const at::Tensor* t : tensors)                                       // undefined without a tangent, and while forward mode is off
+        TORCH_CHECK(t == nullptr || !t->_fw_grad(0).defined(), what, " no forward-mode derivative: unpack the dual tensors first");
     if (!at::GradMode::is_enabled()) return;
     for (const at::Tensor* t : tensors)
         TORCH_CHECK(t == nullptr || !t->requires_grad(), what, " no backward pass: detach the inputs or call under torch.no_grad()");

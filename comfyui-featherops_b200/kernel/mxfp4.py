@@ -12,8 +12,8 @@ every 128 rows x 4 blocks (the byte of row r and block j of a tile is at (r % 32
 largest power of two not above max|x| / 4 as a block's scale, rounds to nearest even and saturates; a block that holds a NaN or an
 infinity becomes NaN.  Sums are fp32 and the result is rounded once.
 
-The operators serve: they have no backward pass, and a call with an input that requires a gradient is refused while gradients are
-enabled.  The reference (fp8e5m2 weights, per-tensor scale) has no such format.
+The operators serve: they have no derivatives.  A call with an input that requires a gradient is refused while gradients are enabled, one
+with a dual tensor of forward-mode differentiation always.  The reference (fp8e5m2 weights, per-tensor scale) has no such format.
 """
 
 import torch

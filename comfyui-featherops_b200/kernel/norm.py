@@ -7,8 +7,8 @@
 r is the residual stream after the block, h what the next block's first linear reads; with `packed=True` h leaves as the MXFP4
 operand of that linear.  Statistics are fp32 and taken over r before it is rounded.
 
-The operator serves: it has no backward pass, and a call with an input that requires a gradient is refused while gradients are
-enabled.  The reference has no norm; a model around it runs these as five to ten elementwise passes.
+The operator serves: it has no derivatives.  A call with an input that requires a gradient is refused while gradients are enabled, one with a
+dual tensor of forward-mode differentiation always.  The reference has no norm; a model around it runs these as five to ten elementwise passes.
 """
 
 import torch

@@ -50,3 +50,28 @@ def test_product_into_a_given_output(native):
                 native.mxfp4_mm_into(*args)
         with pytest.raises(RuntimeError, match="no backward"):
             native.mxfp4_mm_into(a, sa, b, sb, None, out(4, 200).requires_grad_())
+
+
+def test_forward_mode_inputs_are_refused(mx, norm):
+    """The tangent of a dual tensor would be dropped without a word; gradients being off does not turn forward mode off."""
+    import torch.autograd.forward_ad as fwad
+
+    x, bias = torch.ones((4, 64)), torch.ones(64)
+    for no_grad in (False, True):
+        with fwad.dual_level(), torch.set_grad_enabled(not no_grad):
+            dual, dual_bias = fwad.make_dual(x, torch.ones_like(x)), fwad.make_dual(bias, torch.ones_like(bias))
+            u8 = torch.zeros((4, 32), dtype=torch.uint8)
+            for call in (
+                lambda: mx.quantize_mxfp4(dual),
+                lambda: mx.linear_mxfp4(dual, u8, u8),
+                lambda: mx.linear_mxfp4(x, u8, u8, dual_bias),
+                lambda: mx.scaled_mm_mxfp4(u8, u8, u8, u8, dual_bias),
+                lambda: norm.gated_residual_norm(dual),
+                lambda: norm.gated_residual_norm(x, dual),
+                lambda: norm.gated_residual_norm(x, x, gate=dual_bias),
+                lambda: norm.gated_residual_norm(x, x, shift=dual_bias),
+            ):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
+    with fwad.dual_level(), pytest.raises(RuntimeError, match="CUDA"):       # a tensor without a tangent goes on to the other checks
+        mx.quantize_mxfp4(x)
