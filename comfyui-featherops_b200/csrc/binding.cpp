@@ -3,11 +3,16 @@
 // These operators run in a few microseconds on the GPU, less than the same steps take in Python (linear_mxfp4 for one token: 27 us
 // of host time through ctypes).  The kernels stay behind the C ABI of libfeather_b200.so: `bind` takes the addresses of its entry
 // points, so this module links against torch only.  A call releases the GIL while it allocates and launches.
+//
+// A call does not pass torch's dispatcher.  Where somebody watches that (a tracer, a dispatch mode, a functorch transform, a tensor that is
+// a subclass with its own dispatch), it returns NotImplemented once its checks are done, and the caller takes the registered operator, whose
+// implementation comes back here with `direct`.
 #include <Python.h>
 
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -68,6 +73,25 @@ void refuse_grad(std::initializer_list<const at::Tensor*> tensors, const char* w
     for (const at::Tensor* t : tensors)
         TORCH_CHECK(t == nullptr || !t->requires_grad(), what, " no backward pass: detach the inputs or call under torch.no_grad()");
 }
+
+bool has_own_dispatch(const at::Tensor& t) { return t.key_set().has(c10::DispatchKey::Python); }
+
+// Whether the call has to go through the dispatcher.
+bool watched(std::initializer_list<const at::Tensor*> tensors) {
+    constexpr c10::DispatchKeySet watchers({c10::DispatchKey::Tracer, c10::DispatchKey::Python, c10::DispatchKey::PreDispatch, c10::DispatchKey::FuncTorchDynamicLayerFrontMode});
+    const auto tls = c10::impl::tls_local_dispatch_key_set();
+    if (((tls.included_ - tls.excluded_) & watchers) != c10::DispatchKeySet()) return true;
+    for (const at::Tensor* t : tensors)
+        if (t != nullptr && has_own_dispatch(*t)) return true;
+    return false;
+}
+// Sizes that are symbols cannot be checked here.
+bool symbolic(std::initializer_list<const at::Tensor*> tensors) {
+    for (const at::Tensor* t : tensors)
+        if (t != nullptr && t->unsafeGetTensorImpl()->has_symbolic_sizes_strides()) return true;
+    return false;
+}
+PyObject* not_implemented() { Py_RETURN_NOTIMPLEMENTED; }
 
 int* status_word(int device) {
     TORCH_CHECK(device >= 0 && device < kMaxDevices, "device index out of range");
@@ -130,7 +154,7 @@ Packed packed(const at::Tensor& data, const at::Tensor& scales, const char* what
     TORCH_CHECK(data.is_cuda() && scales.is_cuda(), what, " and its scales must be CUDA tensors");
     TORCH_CHECK(scales.device() == data.device(), what, "_scales must be on the same device as ", what);
     TORCH_CHECK(data.is_contiguous() && scales.is_contiguous(), what, " and its scales must be contiguous");
-    TORCH_CHECK(aligned16(data.data_ptr()) && aligned16(scales.data_ptr()), what, " and its scales must be 16-byte aligned");
+    TORCH_CHECK((has_own_dispatch(data) || aligned16(data.data_ptr())) && (has_own_dispatch(scales) || aligned16(scales.data_ptr())), what, " and its scales must be 16-byte aligned");
     return {data, scales, rows, k};
 }
 
@@ -141,11 +165,14 @@ void check_source(const at::Tensor& x) {
 
 PyObject* py_quantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    TORCH_CHECK(n == 1, "quantize(x)");
+    TORCH_CHECK(n == 1 || n == 2, "quantize(x[, direct])");
+    const bool direct = n == 2;
     const at::Tensor& x = tensor(args[0], "x");
     refuse_grad({&x}, "MXFP4 operators have");
+    if (!direct && symbolic({&x})) return not_implemented();
     check_source(x);
     TORCH_CHECK(x.dim() == 2 && x.size(1) != 0 && x.size(1) % 32 == 0, "MXFP4 needs a 2D tensor with K a positive multiple of 32, got ", x.sizes());
+    if (!direct && watched({&x})) return not_implemented();
     const int64_t rows = x.size(0), k = x.size(1);
     at::Tensor data, scales;
     int status = FEATHER_OK;
@@ -171,10 +198,14 @@ PyObject* py_quantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 PyObject* py_dequantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    TORCH_CHECK(n == 3, "dequantize(data, scales, dtype)");
+    TORCH_CHECK(n == 3 || n == 4, "dequantize(data, scales, dtype[, direct])");
+    const bool direct = n == 4;
     const auto dtype = optional_dtype(args[2], "dtype");
     TORCH_CHECK(dtype && source_code(*dtype) >= 0, "dtype must be float32, bfloat16 or float16");
-    const Packed a = packed(tensor(args[0], "data"), tensor(args[1], "scales"), "data");
+    const at::Tensor &data = tensor(args[0], "data"), &scales = tensor(args[1], "scales");
+    if (!direct && symbolic({&data, &scales})) return not_implemented();
+    const Packed a = packed(data, scales, "data");
+    if (!direct && watched({&data, &scales})) return not_implemented();
     at::Tensor out;
     int status = FEATHER_OK;
     {
@@ -209,13 +240,16 @@ int launch_product(const uint8_t* a, const uint8_t* a_scales, const Packed& b, c
 
 PyObject* py_mm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    TORCH_CHECK(n == 6 || n == 7, "mm(a, a_scales, b, b_scales, bias, out_dtype[, out])");
+    TORCH_CHECK(n == 6 || n == 7, "mm(a, a_scales, b, b_scales, bias, out_dtype[, out or None])");
+    const bool direct = n == 7;
     const at::Tensor* const bias = optional_tensor(args[4], "bias");
     const auto out_dtype = optional_dtype(args[5], "out_dtype");
     const at::Tensor* const given = n == 7 ? optional_tensor(args[6], "out") : nullptr;
     refuse_grad({bias, given}, "MXFP4 operators have");
     TORCH_CHECK(out_dtype && (*out_dtype == at::kHalf || *out_dtype == at::kBFloat16), "out_dtype must be float16 or bfloat16");
-    const Packed a = packed(tensor(args[0], "a"), tensor(args[1], "a_scales"), "a"), b = packed(tensor(args[2], "b"), tensor(args[3], "b_scales"), "b");
+    const at::Tensor &a_data = tensor(args[0], "a"), &a_scales = tensor(args[1], "a_scales"), &b_data = tensor(args[2], "b"), &b_scales = tensor(args[3], "b_scales");
+    if (!direct && symbolic({&a_data, &a_scales, &b_data, &b_scales, bias})) return not_implemented();
+    const Packed a = packed(a_data, a_scales, "a"), b = packed(b_data, b_scales, "b");
     const at::Device device = a.data.device();
     check_product(device, a.k, b, bias, out_dtype);
     int64_t ldc = b.rows;
@@ -227,6 +261,7 @@ PyObject* py_mm(PyObject*, PyObject* const* args, Py_ssize_t n) {
         TORCH_CHECK(a.rows <= 1 || given->stride(0) >= b.rows, "rows of out overlap");
         if (a.rows > 1) ldc = given->stride(0);
     }
+    if (!direct && watched({&a_data, &a_scales, &b_data, &b_scales, bias})) return not_implemented();
     int* const status_dev = status_word(device.index());
     at::Tensor out;
     int status = FEATHER_OK;
@@ -244,20 +279,24 @@ PyObject* py_mm(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    TORCH_CHECK(n == 5, "linear(x, b, b_scales, bias, out_dtype)");
+    TORCH_CHECK(n == 5 || n == 6, "linear(x, b, b_scales, bias, out_dtype[, direct])");
+    const bool direct = n == 6;
     const at::Tensor& x = tensor(args[0], "x");
     const at::Tensor* const bias = optional_tensor(args[3], "bias");
     auto out_dtype = optional_dtype(args[4], "out_dtype");
     refuse_grad({&x, bias}, "MXFP4 operators have");
+    const at::Tensor &b_data = tensor(args[1], "b"), &b_scales = tensor(args[2], "b_scales");
+    if (!direct && symbolic({&x, &b_data, &b_scales, bias})) return not_implemented();
     TORCH_CHECK(x.dim() != 0, "x must have at least one dimension");
     check_source(x);
     if (!out_dtype) out_dtype = x.scalar_type() == at::kFloat ? at::kBFloat16 : x.scalar_type();
     TORCH_CHECK(*out_dtype == at::kHalf || *out_dtype == at::kBFloat16, "out_dtype must be float16 or bfloat16");
     const int64_t k = x.size(-1);
     TORCH_CHECK(k != 0 && k % 32 == 0, "x: K must be a positive multiple of 32, got ", k);
-    const Packed b = packed(tensor(args[1], "b"), tensor(args[2], "b_scales"), "b");
+    const Packed b = packed(b_data, b_scales, "b");
     const at::Device device = x.device();
     check_product(device, k, b, bias, out_dtype);
+    if (!direct && watched({&x, &b_data, &b_scales, bias})) return not_implemented();
     int* const status_dev = status_word(device.index());
     const int64_t m = x.numel() / k;
     at::Tensor out;
@@ -328,7 +367,8 @@ Rows aligned_rows(const at::Tensor& t, int64_t cols, bool align) {
 
 PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    TORCH_CHECK(n == 15, "norm(x, y, gate, residual_scale, post_norm, post_weight, weight, bias, scale, shift, kind, eps, out_dtype, want_norm, packed)");
+    TORCH_CHECK(n == 15 || n == 16, "norm(x, y, gate, residual_scale, post_norm, post_weight, weight, bias, scale, shift, kind, eps, out_dtype, want_norm, packed[, direct])");
+    const bool direct = n == 16;
     const at::Tensor& x = tensor(args[0], "x");
     const at::Tensor *const y = optional_tensor(args[1], "y"), *const gate = optional_tensor(args[2], "gate"), *const post_weight = optional_tensor(args[5], "post_weight"),
                      *const weight = optional_tensor(args[6], "weight"), *const bias = optional_tensor(args[7], "bias"), *const scale = optional_tensor(args[8], "scale"),
@@ -337,6 +377,7 @@ PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const bool post_norm = PyObject_IsTrue(args[4]) == 1, want_norm = PyObject_IsTrue(args[13]) == 1, pack = PyObject_IsTrue(args[14]) == 1;
     auto out_dtype = optional_dtype(args[12], "out_dtype");
     refuse_grad({&x, y, gate, post_weight, weight, bias, scale, shift}, "gated_residual_norm has");
+    if (!direct && symbolic({&x, y, gate, post_weight, weight, bias, scale, shift})) return not_implemented();
     TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
     TORCH_CHECK(source_code(x.scalar_type()) >= 0, "x must be float32, bfloat16 or float16");
     TORCH_CHECK(x.dim() != 0 && x.size(-1) != 0, "x must have at least one element in its last dimension");
@@ -370,6 +411,7 @@ PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.gate_rows = check_modulation(gate, "gate", x);
     a.scale_rows = check_modulation(scale, "scale", x);
     a.shift_rows = check_modulation(shift, "shift", x);
+    if (!direct && watched({&x, y, gate, post_weight, weight, bias, scale, shift})) return not_implemented();
     a.status_dev = status_word(device.index());
 
     at::Tensor r, h, h_scales;

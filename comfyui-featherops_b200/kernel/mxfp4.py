@@ -27,10 +27,13 @@ def _tiles(rows, k):
 
 # ------------------------------------------------------------------------------------------------
 # format
+#
+# An operator is one call into the binding; where torch's dispatcher is watched (torch.compile, jit.trace, make_fx, a fake tensor, a dispatch
+# mode) the binding says NotImplemented and the registered operator is called, which the watcher sees.
 # ------------------------------------------------------------------------------------------------
 @torch.library.custom_op("feather_ops_internal::quantize_mxfp4", mutates_args=())
 def _quantize_op(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    return native.binding().quantize(x)
+    return native.binding().quantize(x, True)
 
 
 @_quantize_op.register_fake
@@ -42,12 +45,13 @@ def _(x):
 def quantize_mxfp4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """x [R, K] fp32 / bf16 / fp16 on the GPU, K % 32 == 0 -> (data uint8 [R, K/2], scales uint8 [ceil(R/128), ceil(K/128), 512]).
     Rows may be strided; a tensor whose columns are strided is copied first.  Scale bytes of rows past R are not written."""
-    return _quantize_op(x) if torch.compiler.is_compiling() else native.binding().quantize(x)
+    out = NotImplemented if torch.compiler.is_compiling() else native.binding().quantize(x)
+    return _quantize_op(x) if out is NotImplemented else out
 
 
 @torch.library.custom_op("feather_ops_internal::dequantize_mxfp4", mutates_args=())
 def _dequantize_op(data: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    return native.binding().dequantize(data, scales, dtype)
+    return native.binding().dequantize(data, scales, dtype, True)
 
 
 @_dequantize_op.register_fake
@@ -57,7 +61,8 @@ def _(data, scales, dtype):
 
 def dequantize_mxfp4(data: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     """The values MXFP4 rows stand for, rounded once to `dtype` (exact in fp32 and, for scales from 2^-125 on, in bf16)."""
-    return _dequantize_op(data, scales, dtype) if torch.compiler.is_compiling() else native.binding().dequantize(data, scales, dtype)
+    out = NotImplemented if torch.compiler.is_compiling() else native.binding().dequantize(data, scales, dtype)
+    return _dequantize_op(data, scales, dtype) if out is NotImplemented else out
 
 
 def prepack_mxfp4_scales(scales: torch.Tensor) -> torch.Tensor:
@@ -85,7 +90,7 @@ def unprepack_mxfp4_scales(scales: torch.Tensor, rows: int, k: int) -> torch.Ten
 # ------------------------------------------------------------------------------------------------
 @torch.library.custom_op("feather_ops_internal::scaled_mm_mxfp4", mutates_args=())
 def _mm_op(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, bias: torch.Tensor | None, out_dtype: torch.dtype) -> torch.Tensor:
-    return native.binding().mm(a, a_scales, b, b_scales, bias, out_dtype)
+    return native.binding().mm(a, a_scales, b, b_scales, bias, out_dtype, None)
 
 
 @_mm_op.register_fake
@@ -96,14 +101,13 @@ def _(a, a_scales, b, b_scales, bias, out_dtype):
 def scaled_mm_mxfp4(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, bias: torch.Tensor | None = None,
                     out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """round(a @ b^T + bias): a [M, K] and b [N, K] in MXFP4 (`quantize_mxfp4`), bias [N] of out_dtype, result [M, N] fp16 / bf16."""
-    if torch.compiler.is_compiling():
-        return _mm_op(a, a_scales, b, b_scales, bias, out_dtype)
-    return native.binding().mm(a, a_scales, b, b_scales, bias, out_dtype)
+    out = NotImplemented if torch.compiler.is_compiling() else native.binding().mm(a, a_scales, b, b_scales, bias, out_dtype)
+    return _mm_op(a, a_scales, b, b_scales, bias, out_dtype) if out is NotImplemented else out
 
 
 @torch.library.custom_op("feather_ops_internal::linear_mxfp4", mutates_args=())
 def _linear_op(x: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, bias: torch.Tensor | None, out_dtype: torch.dtype | None) -> torch.Tensor:
-    return native.binding().linear(x, b, b_scales, bias, out_dtype)
+    return native.binding().linear(x, b, b_scales, bias, out_dtype, True)
 
 
 @_linear_op.register_fake
@@ -115,9 +119,8 @@ def _(x, b, b_scales, bias, out_dtype):
 def linear_mxfp4(x: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, bias: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """x [..., K] fp32 / bf16 / fp16 -> [..., N]: the rows of x are quantised to MXFP4 and multiplied with the weight b [N, K].
     out_dtype: fp16 or bf16; by default x's dtype if that is one of them, else bf16."""
-    if torch.compiler.is_compiling():
-        return _linear_op(x, b, b_scales, bias, out_dtype)
-    return native.binding().linear(x, b, b_scales, bias, out_dtype)
+    out = NotImplemented if torch.compiler.is_compiling() else native.binding().linear(x, b, b_scales, bias, out_dtype)
+    return _linear_op(x, b, b_scales, bias, out_dtype) if out is NotImplemented else out
 
 
 class MXFP4Linear:

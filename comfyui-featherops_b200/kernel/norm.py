@@ -35,7 +35,7 @@ def _norm_op(
     packed: bool,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(r, h, scales of h); what a call does not ask for is empty, as is r without y."""
-    r, h = native.binding().norm(x, y, gate, residual_scale, post_norm, post_weight, weight, bias, scale, shift, kind, eps, out_dtype, want_norm, packed)
+    r, h = native.binding().norm(x, y, gate, residual_scale, post_norm, post_weight, weight, bias, scale, shift, kind, eps, out_dtype, want_norm, packed, True)
     h, scales = h if packed else (h, x.new_empty((0,), dtype=torch.uint8))
     return r if y is not None else x.new_empty((0,)), h if h is not None else x.new_empty((0,), dtype=out_dtype), scales
 
@@ -61,11 +61,13 @@ def gated_residual_norm(x, y=None, gate=None, residual_scale=1.0, post_norm=Fals
     out_dtype: h's dtype (default: the 16-bit one of x and y, x's first).  packed=True: h is the pair (data, scales) that
     `quantize_mxfp4` gives for the [rows, C] h of out_dtype, bit for bit.
     """
-    if torch.compiler.is_compiling():
-        if out_dtype is None:
-            out_dtype = x.dtype if x.dtype != torch.float32 or y is None else y.dtype
-            if packed and out_dtype == torch.float32:
-                out_dtype = torch.bfloat16
-        r, h, scales = _norm_op(x, y, gate, float(residual_scale), post_norm, post_weight, weight, bias, scale, shift, kind, float(eps), out_dtype, want_norm, packed)
-        return (x if y is None else r), ((h, scales) if packed else h if want_norm else None)
-    return native.binding().norm(x, y, gate, residual_scale, post_norm, post_weight, weight, bias, scale, shift, kind, eps, out_dtype, want_norm, packed)
+    if not torch.compiler.is_compiling():
+        out = native.binding().norm(x, y, gate, residual_scale, post_norm, post_weight, weight, bias, scale, shift, kind, eps, out_dtype, want_norm, packed)
+        if out is not NotImplemented:
+            return out
+    if out_dtype is None:                                                   # through the dispatcher, for whoever watches it (kernel/mxfp4.py)
+        out_dtype = x.dtype if x.dtype != torch.float32 or y is None else y.dtype
+        if packed and out_dtype == torch.float32:
+            out_dtype = torch.bfloat16
+    r, h, scales = _norm_op(x, y, gate, float(residual_scale), post_norm, post_weight, weight, bias, scale, shift, kind, float(eps), out_dtype, want_norm, packed)
+    return (x if y is None else r), ((h, scales) if packed else h if want_norm else None)
