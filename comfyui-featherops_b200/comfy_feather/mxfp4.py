@@ -66,9 +66,15 @@ class FeatherMXFP4Layout(QuantizedLayout):
 
 
 def scaled_weight(weight, scale):
-    """The values of a scaled checkpoint weight, in fp32."""
+    """The values of a scaled checkpoint weight, in fp32; scale: one element, or a column of one for each row of the weight."""
     weight = weight.to(torch.float32)
-    return weight if scale is None else weight * scale.to(device=weight.device, dtype=torch.float32)
+    if scale is None:
+        return weight
+    if scale.numel() == 1:
+        scale = scale.reshape(())
+    elif weight.ndim != 2 or tuple(scale.shape) != (weight.shape[0], 1):
+        raise ValueError(f"the scale of a weight {tuple(weight.shape)} has one element or a column of one for each row, got {tuple(scale.shape)}")
+    return weight * scale.to(device=weight.device, dtype=torch.float32)
 
 
 def make_mxfp4_weight(weight, scale, orig_dtype):

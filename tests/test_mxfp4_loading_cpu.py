@@ -38,3 +38,32 @@ def test_a_plain_layer_without_a_scale_is_left_alone(ops_mod):
     for weight in (torch.randn(40, 48), torch.randn(40, 48).to(torch.float8_e5m2)):
         lin = _linear(ops_mod, 48, 40, {"weight": weight})
         assert lin.weight.dtype == weight.dtype and torch.equal(lin.weight.float(), weight.float())
+
+
+def _unscaled(monkeypatch, layout):
+    """The fp32 weight that would be quantised, instead of quantising it."""
+    seen = []
+
+    def quantize(x):
+        seen.append(x)
+        return torch.zeros((x.shape[0], x.shape[1] // 2), dtype=torch.uint8), torch.zeros((1, 1, 512), dtype=torch.uint8)
+
+    monkeypatch.setattr(layout, "_quantize", quantize)
+    return seen
+
+
+def test_which_axis_a_scale_belongs_to(ops_mod, monkeypatch):
+    """One scale, or one for each output row as a column; anything else would be spread along K or over a wrong axis."""
+    layout = importlib.import_module("feather_b200.comfy_feather.mxfp4")
+    seen = _unscaled(monkeypatch, layout)
+    w = torch.randn((64, 64)).to(torch.float8_e4m3fn)
+    for scale in (torch.tensor(0.5), torch.tensor([0.5]), torch.rand(64, 1)):
+        layout.make_mxfp4_weight(w, scale, torch.bfloat16)
+        assert torch.equal(seen.pop(), w.float() * scale.reshape(-1, 1))
+    for scale in (torch.rand(64), torch.rand(1, 64), torch.rand(64, 64), torch.rand(64, 2), torch.rand(1, 64, 1)):
+        with pytest.raises(ValueError, match="scale"):
+            layout.make_mxfp4_weight(w, scale, torch.bfloat16)
+        with pytest.raises(ValueError, match="scale"):
+            _linear(ops_mod, 64, 64, {"weight": w, "weight_scale": scale}, ("ffn",))
+    vector = _linear(ops_mod, 1, 8, {"weight": torch.ones(8).to(torch.float8_e5m2), "weight_scale": torch.tensor([2.0])})
+    assert torch.equal(vector.weight, torch.full((8,), 2.0, dtype=torch.bfloat16))
