@@ -83,8 +83,8 @@ def make_mxfp4_weight(weight, scale, orig_dtype):
         raise ValueError(f"MXFP4 weights require a 2D tensor, got {weight.ndim}D")
     if weight.dtype == torch.uint8:
         n, k = weight.shape[0], weight.shape[1] * 2
-        if scale is None or scale.element_size() != 1 or tuple(scale.shape) != (n, k // 32) or k % 32 != 0:
-            raise ValueError(f"a packed MXFP4 weight {tuple(weight.shape)} needs E8M0 scale bytes of shape {(n, k // 32)}")
+        if scale is None or scale.dtype not in mxfp4.SCALE_DTYPES or tuple(scale.shape) != (n, k // 32) or k % 32 != 0:
+            raise ValueError(f"a packed MXFP4 weight {tuple(weight.shape)} needs E8M0 scale bytes (uint8 or float8_e8m0fnu) of shape {(n, k // 32)}")
         params = FeatherMXFP4Params(scale=mxfp4.prepack_mxfp4_scales(scale.to(weight.device)), orig_dtype=orig_dtype, orig_shape=(n, k))
         return QuantizedTensor(weight.contiguous(), FEATHER_MXFP4_LAYOUT, params)
     if scale is not None or weight.dtype not in _SOURCES:

@@ -21,6 +21,9 @@ import torch
 from .b200 import native
 
 
+SCALE_DTYPES = (torch.uint8, torch.float8_e8m0fnu)                          # what E8M0 bytes are stored as
+
+
 def _tiles(rows, k):
     return ((rows + 127) // 128, (k + 127) // 128, 512)
 
@@ -67,8 +70,8 @@ def dequantize_mxfp4(data: torch.Tensor, scales: torch.Tensor, dtype: torch.dtyp
 
 def prepack_mxfp4_scales(scales: torch.Tensor) -> torch.Tensor:
     """E8M0 scale bytes [R, K/32] as a checkpoint stores them -> [ceil(R/128), ceil(K/128), 512] tiles, padded with zeros."""
-    if scales.dim() != 2 or scales.element_size() != 1:
-        raise RuntimeError("scales must be a 2D tensor of bytes [rows, K/32]")
+    if scales.dim() != 2 or scales.dtype not in SCALE_DTYPES:
+        raise RuntimeError(f"scales must be a 2D tensor of E8M0 bytes [rows, K/32] (uint8 or float8_e8m0fnu), got {scales.dtype} {list(scales.shape)}")
     scales = scales.contiguous().view(torch.uint8)
     rows, blocks = scales.shape
     tr, tk, _ = _tiles(rows, blocks * 32)

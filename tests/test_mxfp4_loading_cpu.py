@@ -67,3 +67,17 @@ def test_which_axis_a_scale_belongs_to(ops_mod, monkeypatch):
             _linear(ops_mod, 64, 64, {"weight": w, "weight_scale": scale}, ("ffn",))
     vector = _linear(ops_mod, 1, 8, {"weight": torch.ones(8).to(torch.float8_e5m2), "weight_scale": torch.tensor([2.0])})
     assert torch.equal(vector.weight, torch.full((8,), 2.0, dtype=torch.bfloat16))
+
+
+def test_packed_scales_are_e8m0(pkg):
+    """Bytes of another format are no exponents: 0x38 is 1.0 as e4m3 and 2^-71 as E8M0."""
+    layout = importlib.import_module("feather_b200.comfy_feather.mxfp4")
+    mx = importlib.import_module("feather_b200.kernel.mxfp4")
+    data, ones = torch.zeros((8, 32), dtype=torch.uint8), torch.ones((8, 2))
+    for scale in (torch.full((8, 2), 127, dtype=torch.uint8), ones.to(torch.float8_e8m0fnu)):
+        assert layout.make_mxfp4_weight(data, scale, torch.bfloat16)._params.scale.view(-1)[0] == 127
+    for dtype in (torch.float8_e4m3fn, torch.float8_e5m2, torch.int8, torch.bool):
+        with pytest.raises(ValueError, match="scale bytes"):
+            layout.make_mxfp4_weight(data, ones.to(dtype), torch.bfloat16)
+        with pytest.raises(RuntimeError, match="bytes"):
+            mx.prepack_mxfp4_scales(ones.to(dtype))
