@@ -86,7 +86,10 @@ def make_mxfp4_weight(weight, scale, orig_dtype):
         if scale is None or scale.dtype not in mxfp4.SCALE_DTYPES or tuple(scale.shape) != (n, k // 32) or k % 32 != 0:
             raise ValueError(f"a packed MXFP4 weight {tuple(weight.shape)} needs E8M0 scale bytes (uint8 or float8_e8m0fnu) of shape {(n, k // 32)}")
         params = FeatherMXFP4Params(scale=mxfp4.prepack_mxfp4_scales(scale.to(weight.device)), orig_dtype=orig_dtype, orig_shape=(n, k))
-        return QuantizedTensor(weight.contiguous(), FEATHER_MXFP4_LAYOUT, params)
+        weight = weight.contiguous()
+        if weight.data_ptr() % 16 != 0:                            # a view into a loader's buffer; the kernels need 16-byte alignment
+            weight = weight.clone()
+        return QuantizedTensor(weight, FEATHER_MXFP4_LAYOUT, params)
     if scale is not None or weight.dtype not in _SOURCES:
         weight = scaled_weight(weight, scale)
     data, scales = _quantize(weight)

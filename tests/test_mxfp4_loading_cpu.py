@@ -81,3 +81,17 @@ def test_packed_scales_are_e8m0(pkg):
             layout.make_mxfp4_weight(data, ones.to(dtype), torch.bfloat16)
         with pytest.raises(RuntimeError, match="bytes"):
             mx.prepack_mxfp4_scales(ones.to(dtype))
+
+
+def test_a_packed_weight_that_lies_unaligned_is_copied(pkg):
+    """A loader may hand out views of one buffer at any offset; the kernels read 16 bytes at a time."""
+    layout = importlib.import_module("feather_b200.comfy_feather.mxfp4")
+    n, k = 40, 96
+    scale = torch.full((n, k // 32), 127, dtype=torch.uint8)
+    buffer = torch.randint(0, 256, (n * k // 2 + 64,), generator=torch.Generator().manual_seed(1)).to(torch.uint8)
+    first = (-buffer.data_ptr()) % 16
+    for offset in range(17):
+        view = buffer[first + offset:first + offset + n * k // 2].view(n, k // 2)
+        weight = layout.make_mxfp4_weight(view, scale, torch.bfloat16)
+        assert weight._qdata.data_ptr() % 16 == 0 and weight._qdata.is_contiguous() and torch.equal(weight._qdata, view)
+        assert (weight._qdata.data_ptr() == view.data_ptr()) == (offset % 16 == 0)       # no copy where none is needed
