@@ -60,6 +60,11 @@ double number(PyObject* o) {
     if (v == -1.0 && PyErr_Occurred()) throw python_error();
     return v;
 }
+bool truth(PyObject* o) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw python_error();
+    return v == 1;
+}
 
 int source_code(at::ScalarType t) {
     return t == at::kFloat ? FEATHER_SRC_FP32 : t == at::kBFloat16 ? FEATHER_SRC_BF16 : t == at::kHalf ? FEATHER_SRC_FP16 : -1;
@@ -374,7 +379,7 @@ PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
                      *const weight = optional_tensor(args[6], "weight"), *const bias = optional_tensor(args[7], "bias"), *const scale = optional_tensor(args[8], "scale"),
                      *const shift = optional_tensor(args[9], "shift");
     const double residual_scale = number(args[3]), eps = number(args[11]);
-    const bool post_norm = PyObject_IsTrue(args[4]) == 1, want_norm = PyObject_IsTrue(args[13]) == 1, pack = PyObject_IsTrue(args[14]) == 1;
+    const bool post_norm = truth(args[4]), want_norm = truth(args[13]), pack = truth(args[14]);
     auto out_dtype = optional_dtype(args[12], "out_dtype");
     refuse_grad({&x, y, gate, post_weight, weight, bias, scale, shift}, "gated_residual_norm has");
     if (!direct && symbolic({&x, y, gate, post_weight, weight, bias, scale, shift})) return not_implemented();

@@ -75,3 +75,14 @@ def test_forward_mode_inputs_are_refused(mx, norm):
                     call()
     with fwad.dual_level(), pytest.raises(RuntimeError, match="CUDA"):       # a tensor without a tangent goes on to the other checks
         mx.quantize_mxfp4(x)
+
+
+def test_flags_that_have_no_truth_value(norm):
+    """The error of the flag itself, not one of the interpreter's about an error that was left behind."""
+    x = torch.zeros((2, 64))
+    for name in ("post_norm", "want_norm", "packed"):
+        with pytest.raises(RuntimeError, match="ambiguous"):
+            norm.gated_residual_norm(x, **{name: torch.tensor([1, 2])})
+    for name in ("residual_scale", "eps"):
+        with pytest.raises(TypeError):
+            norm.gated_residual_norm(x, **{name: "much"})
