@@ -126,7 +126,7 @@ Rows rows_of(const at::Tensor& t, int64_t cols) {
     const auto sizes = t.sizes();
     const auto strides = t.strides();
     int64_t ld = cols, count = 1, next = -1;
-    bool ok = strides.back() == 1 || cols == 1;
+    bool ok = (strides.back() == 1 || cols == 1) && !t.is_neg();
     for (int64_t d = t.dim() - 2; ok && d >= 0; --d) {
         if (sizes[d] == 1) continue;
         if (next < 0) ld = strides[d];
@@ -135,7 +135,7 @@ Rows rows_of(const at::Tensor& t, int64_t cols) {
         count *= sizes[d];
     }
     if (ok && (count <= 1 || ld >= cols)) return {at::Tensor(), t.data_ptr(), ld};
-    at::Tensor copy = t.contiguous();
+    at::Tensor copy = t.clone(at::MemoryFormat::Contiguous).resolve_neg();
     void* const p = copy.data_ptr();
     return {std::move(copy), p, cols};
 }
@@ -235,6 +235,7 @@ void check_product(const at::Device& device, int64_t k, const Packed& b, const a
         TORCH_CHECK(bias->device() == device, "bias must be on the same device as a");
         TORCH_CHECK(bias->scalar_type() == *out_dtype, "bias must have the out dtype");
         TORCH_CHECK(bias->numel() == b.rows && bias->is_contiguous(), "bias must be contiguous with N elements");
+        TORCH_CHECK(!bias->is_neg(), "bias carries its sign as a flag: resolve_neg() it first");
     }
 }
 
@@ -263,6 +264,7 @@ PyObject* py_mm(PyObject*, PyObject* const* args, Py_ssize_t n) {
         TORCH_CHECK(given->scalar_type() == *out_dtype, "out must have the out dtype");
         TORCH_CHECK(given->dim() == 2 && given->size(0) == a.rows && given->size(1) == b.rows, "out must be [", a.rows, ", ", b.rows, "], got ", given->sizes());
         TORCH_CHECK(b.rows == 1 || given->stride(1) == 1, "out must have contiguous columns");
+        TORCH_CHECK(!given->is_neg(), "out carries its sign as a flag: resolve_neg() it first");
         TORCH_CHECK(a.rows <= 1 || given->stride(0) >= b.rows, "rows of out overlap");
         if (a.rows > 1) ldc = given->stride(0);
     }
