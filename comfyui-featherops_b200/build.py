@@ -1,15 +1,18 @@
 """Builds libfeather_b200.so (the C-ABI library declared in include/feather_b200.h) in-tree with nvcc for sm_100a, and
-_feather_binding.so (the torch binding of the MXFP4 operators and the fused norm, csrc/binding.cpp) with the C++ compiler.
+the torch binding of the MXFP4 operators and the fused norm (csrc/binding.cpp) with the C++ compiler.  The binding's file name carries
+the Python and the torch it is for; where its tools are missing (``binding_unavailable()``) only the library is built.
 
-Usage: ``python build.py`` from any directory, or ``build_library()`` and ``build_binding()`` from Python.  nvcc cross-compiles, so no GPU is
+Usage: ``python build.py`` from any directory, or ``build_all()``, ``build_library()`` and ``build_binding()`` from Python.  nvcc cross-compiles, so no GPU is
 needed to build.  The library links the CUDA runtime statically and resolves the one driver symbol it needs
 (cuTensorMapEncodeTiled) at run time, so it also loads on a machine without a driver (every call then reports an error).
 """
 
+import importlib.machinery
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC_DIR = os.path.join(PKG_DIR, "csrc")
@@ -80,34 +83,69 @@ def build_library(force=False, verbose=False):
 
 
 BINDING_SRC = os.path.join(CSRC_DIR, "binding.cpp")
-BINDING_PATH = os.path.join(PKG_DIR, "_feather_binding.so")
+
+
+def binding_path():
+    """Where the binding for this Python and this torch lies (the loader, kernel/b200/native.py, means the same file)."""
+    import torch
+
+    return os.path.join(PKG_DIR, f"_feather_binding.torch-{torch.__version__}{importlib.machinery.EXTENSION_SUFFIXES[0]}")
+
+
+def _cxx():
+    return shutil.which("c++") or shutil.which("g++")
+
+
+def binding_unavailable():
+    """What this machine lacks to build the binding, or None.  The library and the fp8 linear need none of it."""
+    try:
+        import torch
+    except ImportError:
+        return "torch is not installed"
+    if _cxx() is None:
+        return "there is no C++ compiler"
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        return "the headers of Python are not installed"
+    if not os.path.exists(os.path.join(os.path.dirname(torch.__file__), "include", "ATen", "core", "Tensor.h")):
+        return "the headers of torch are not installed"
+    return None
 
 
 def build_binding(force=False):
-    """Compile csrc/binding.cpp against the installed torch into _feather_binding.so.  Returns its path.  The module takes the
-    entry points of libfeather_b200.so as addresses when it is loaded, so the two are built independently."""
-    import sysconfig
-
+    """Compile csrc/binding.cpp against the installed torch.  Returns the path.  The module takes the entry points of
+    libfeather_b200.so as addresses when it is loaded, so the two are built independently."""
     import torch
 
+    path, cxx = binding_path(), _cxx()
     deps = [BINDING_SRC, os.path.join(PKG_DIR, "..", "include", "feather_b200.h"), torch.__file__]
-    if not force and os.path.exists(BINDING_PATH) and all(os.path.getmtime(d) <= os.path.getmtime(BINDING_PATH) for d in deps):
-        return BINDING_PATH
-    cxx = shutil.which("c++") or shutil.which("g++")
-    if cxx is None:
-        raise RuntimeError("no C++ compiler found: _feather_binding.so cannot be built")
+    if not force and os.path.exists(path) and all(os.path.getmtime(d) <= os.path.getmtime(path) for d in deps):
+        return path
+    reason = binding_unavailable()
+    if reason is not None:
+        raise RuntimeError(f"the torch binding cannot be built: {reason}")
     torch_dir = os.path.dirname(torch.__file__)
     include = os.path.join(torch_dir, "include")
     cuda = os.path.dirname(os.path.dirname(_nvcc()))
-    tmp = BINDING_PATH + ".tmp"
+    tmp = path + ".tmp"
     cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-I", include, "-I", os.path.join(include, "torch", "csrc", "api", "include"), "-I", sysconfig.get_paths()["include"], "-I", os.path.join(cuda, "include"),
            BINDING_SRC, "-L", os.path.join(torch_dir, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python", "-o", tmp]
     res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"torch binding failed to build:\n{res.stdout}")
-    os.replace(tmp, BINDING_PATH)
-    return BINDING_PATH
+    os.replace(tmp, path)
+    return path
+
+
+def build_all(force=False, verbose=False):
+    """The library and, where its tools are there, the binding.  Returns their paths."""
+    paths = [build_library(force=force, verbose=verbose)]
+    reason = binding_unavailable()
+    if reason is None:
+        paths.append(build_binding(force=force))
+    else:
+        print(f"torch binding not built: {reason} (the MXFP4 operators and the fused norm will not be available)", file=sys.stderr)
+    return paths
 
 
 CBENCH_SRC = os.path.join(PKG_DIR, "cbench", "bench_scaled_mm.c")
@@ -131,8 +169,7 @@ def build_cbench(cc=None):
 
 
 if __name__ == "__main__":
-    path = build_library(force="--force" in sys.argv, verbose="-v" in sys.argv)
-    print(path)
-    print(build_binding(force="--force" in sys.argv))
+    for path in build_all(force="--force" in sys.argv, verbose="-v" in sys.argv):
+        print(path)
     if "--cbench" in sys.argv:
         print(build_cbench())

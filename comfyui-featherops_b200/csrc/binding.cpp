@@ -18,7 +18,6 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
-#include <torch/version.h>
 
 #include "../../include/feather_b200.h"
 
@@ -527,10 +526,5 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_feather_binding", nullptr, -1, 
 }  // namespace
 
 PyMODINIT_FUNC PyInit__feather_binding() {
-    PyObject* const m = PyModule_Create(&g_module);
-    if (m != nullptr && PyModule_AddStringConstant(m, "torch_version", TORCH_VERSION) != 0) {
-        Py_DECREF(m);
-        return nullptr;
-    }
-    return m;
+    return PyModule_Create(&g_module);
 }

@@ -18,7 +18,12 @@ import torch
 
 _PKG_DIR = os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 LIB_PATH = os.path.join(_PKG_DIR, "libfeather_b200.so")
-BINDING_PATH = os.path.join(_PKG_DIR, "_feather_binding.so")
+
+
+def binding_path():
+    """The binding built for this Python and this torch (build.py names it so): one of others is never loaded."""
+    return os.path.join(_PKG_DIR, f"_feather_binding.torch-{torch.__version__}{importlib.machinery.EXTENSION_SUFFIXES[0]}")
+
 
 FEATHER_OK = 0
 FEATHER_ERR_DEVICE_TIMEOUT = 5
@@ -659,16 +664,15 @@ def _load_binding():
     with _lib_lock:
         if _binding is not None:
             return _binding
-        if not os.path.exists(BINDING_PATH):
+        path = binding_path()
+        if not os.path.exists(path):
             raise FeatherNativeError(
-                f"{BINDING_PATH} is missing. Build it with `python {os.path.join(_PKG_DIR, 'build.py')}` "
+                f"{path} is missing. Build it with `python {os.path.join(_PKG_DIR, 'build.py')}` "
                 "(needs a C++ compiler; there is no fallback implementation)."
             )
-        loader = importlib.machinery.ExtensionFileLoader("_feather_binding", BINDING_PATH)
-        mod = importlib.util.module_from_spec(importlib.util.spec_from_file_location("_feather_binding", BINDING_PATH, loader=loader))
+        loader = importlib.machinery.ExtensionFileLoader("_feather_binding", path)
+        mod = importlib.util.module_from_spec(importlib.util.spec_from_file_location("_feather_binding", path, loader=loader))
         loader.exec_module(mod)
-        if mod.torch_version != torch.__version__.split("+")[0]:
-            raise FeatherNativeError(f"{BINDING_PATH} was built for torch {mod.torch_version}, this is {torch.__version__}: run build.py again")
         entries = (lib.feather_mxfp4_quantize, lib.feather_mxfp4_dequantize, lib.feather_mxfp4_mm, lib.feather_gated_norm, lib.feather_last_error_string)
         mod.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in entries), FeatherNativeError, _status_address)
         _binding = mod
