@@ -5,7 +5,7 @@
 //   h = (norm(r) * weight + bias) * (1 + scale) + shift
 //   norm(v) = v / sqrt(mean(v^2) + eps)      or  (v - mean(v)) / sqrt(var(v) + eps)
 //
-// A row lives in the registers of one warp or one block from its only read to its only write; sums are fp32, over the values as
+// A row lives in the registers of a block, or of one group of a block's threads, from its only read to its only write; sums are fp32, over the values as
 // they are before r is rounded to x's type.  h leaves in 16 or 32 bits or, rounded to 16 bits first, as the MXFP4 operand of the
 // product that follows (mxfp4.cuh).
 #include <cuda_runtime.h>
@@ -130,36 +130,33 @@ __device__ __forceinline__ void values_any(const RawAny& r, int type, float (&v)
 struct NormParams {
     feather_norm_args a;
     int vecs;             // vectors (or elements) of a row
-    int chunk;            // consecutive rows of a warp or block
+    int chunk;            // consecutive rows of a block
     int groups, stages;   // of the kernel for many rows
     float inv_cols;
     uint64_t wait_ns;     // limit of its waits for a row
 };
 
 // ------------------------------------------------------------------------------------------------ sums over a row
-// Sum over the row's threads: one warp (WARP_ROW), or the whole block through `part`.  A buffer is used again two sums later, past
-// the other buffer's barrier, so one barrier for each sum is enough.  Entries past the block's warps are zero (clear_parts).
+// Sum over a row, which is the whole block's, through `part`.  A buffer is used again two sums later, past the other buffer's barrier, so one
+// barrier for each sum is enough.  Entries past the block's warps are zero (clear_parts).
 constexpr int kNormMaxWarps = 32;
 __device__ __forceinline__ void clear_parts(float (*part)[kNormMaxWarps]) {
     for (int i = threadIdx.x; i < 2 * kNormMaxWarps; i += blockDim.x) (&part[0][0])[i] = 0.0f;
     __syncthreads();
 }
-template <bool WARP_ROW>
 __device__ __forceinline__ float row_sum(float v, float (*part)[kNormMaxWarps], int& flip) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if constexpr (!WARP_ROW) {
-        if ((threadIdx.x & 31) == 0) part[flip][threadIdx.x >> 5] = v;
-        __syncthreads();
-        const float4* const q = reinterpret_cast<const float4*>(part[flip]);
-        const int quads = (blockDim.x + 127) >> 7;
-        v = 0.0f;
-        for (int i = 0; i < quads; ++i) {                                     // the same order in every thread
-            const float4 x = q[i];
-            v += (x.x + x.y) + (x.z + x.w);
-        }
-        flip ^= 1;
+    if ((threadIdx.x & 31) == 0) part[flip][threadIdx.x >> 5] = v;
+    __syncthreads();
+    const float4* const q = reinterpret_cast<const float4*>(part[flip]);
+    const int quads = (blockDim.x + 127) >> 7;
+    v = 0.0f;
+    for (int i = 0; i < quads; ++i) {                                         // the same order in every thread
+        const float4 x = q[i];
+        v += (x.x + x.y) + (x.z + x.w);
     }
+    flip ^= 1;
     return v;
 }
 
@@ -239,30 +236,24 @@ __device__ __forceinline__ long long next_change(const feather_norm_args& a, lon
     return change;
 }
 
-// Takes the row's values to v - mean (layer) and returns 1 / sqrt(mean square + eps).  The variance is taken about the mean in a second
-// pass over the registers: sums of squares of unshifted values lose a small variance beside a large mean.
-template <int NV, bool WARP_ROW>
-__device__ __forceinline__ float normalise(float (&v)[NV][8], const NormParams& p, int first, int step, float (*part)[kNormMaxWarps], int& flip) {
+// Takes a thread's vector of the row to v - mean (layer) and returns 1 / sqrt(mean square + eps); in: the vector exists, it holds zeros otherwise.
+// The variance is taken about the mean in a second pass over the registers: sums of squares of unshifted values lose a small variance beside a
+// large mean.
+__device__ __forceinline__ float normalise(float (&v)[8], const NormParams& p, bool in, float (*part)[kNormMaxWarps], int& flip) {
     if (p.a.kind == FEATHER_NORM_LAYER) {
         float s = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int j = 0; j < 8; ++j) s += v[j];
+        const float mean = row_sum(s, part, flip) * p.inv_cols;
+        if (in) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s += v[i][j];                         // vectors past the row hold zeros
-        const float mean = row_sum<WARP_ROW>(s, part, flip) * p.inv_cols;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (first + i * step < p.vecs) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[i][j] -= mean;
-            }
+            for (int j = 0; j < 8; ++j) v[j] -= mean;
+        }
     }
     float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s += v[i][j] * v[i][j];
-    return 1.0f / sqrtf(row_sum<WARP_ROW>(s, part, flip) * p.inv_cols + p.a.eps);
+    for (int j = 0; j < 8; ++j) s += v[j] * v[j];
+    return 1.0f / sqrtf(row_sum(s, part, flip) * p.inv_cols + p.a.eps);
 }
 
 // One vector of h, given n.  All lanes of a warp call this together (the MXFP4 form exchanges between lanes); `in`: the vector exists.
@@ -660,34 +651,34 @@ __global__ void __maxnreg__(DENSE ? 48 : 64) gated_norm_row_kernel(const __grid_
     const bool in = vec < p.vecs;
     const int present = norm_present(a);
     const ModulationAt m = modulation_at(a, row);
-    Raw8<XT> xr[1];
-    Raw8<YT> yr[1];
+    Raw8<XT> xr;
+    Raw8<YT> yr;
     RawAny gate, post_weight;
     if (in) {
         if (a.y != nullptr) {
-            yr[0] = load8<YT>(a.y, row * a.ldy + at);
+            yr = load8<YT>(a.y, row * a.ldy + at);
             load_any(gate, a.gate, a.gate_dtype, m.gate + at);
             load_any(post_weight, a.post_weight, a.post_weight_dtype, at);
         }
-        xr[0] = load8<XT>(a.x, row * a.ldx + at);
+        xr = load8<XT>(a.x, row * a.ldx + at);
     }
     int flip = 0;
-    float v[1][8];
+    float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[0][j] = 0.0f;
+    for (int j = 0; j < 8; ++j) v[j] = 0.0f;
     if (a.y != nullptr) {
-        if (in) values8<YT>(yr[0], v[0]);
-        const float inv = a.post_norm ? normalise<1, false>(v, p, vec, 0, part, flip) : 1.0f;
+        if (in) values8<YT>(yr, v);
+        const float inv = a.post_norm ? normalise(v, p, in, part, flip) : 1.0f;
         if (in) {
             float g[8], x[8];
             fold_g(a, gate, post_weight, g);
-            values8<XT>(xr[0], x);
+            values8<XT>(xr, x);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[0][j] = x[j] + g[j] * (v[0][j] * inv);
-            if (a.r != nullptr) store8<XT>(a.r, row * a.ldr + at, v[0]);
+            for (int j = 0; j < 8; ++j) v[j] = x[j] + g[j] * (v[j] * inv);
+            if (a.r != nullptr) store8<XT>(a.r, row * a.ldr + at, v);
         }
     } else if (in) {
-        values8<XT>(xr[0], v[0]);
+        values8<XT>(xr, v);
     }
     if (a.h == nullptr) return;
     RawAny weight, bias, scale, shift;                                        // on their way during the sums
@@ -697,20 +688,20 @@ __global__ void __maxnreg__(DENSE ? 48 : 64) gated_norm_row_kernel(const __grid_
         load_any(weight, a.weight, a.weight_dtype, at);
         load_any(bias, a.bias, a.bias_dtype, at);
     }
-    const float inv = normalise<1, false>(v, p, vec, 0, part, flip);
+    const float inv = normalise(v, p, in, part, flip);
     if (in) {
         float s[8], u[8];
         start_ab(a, scale, bias, s, u);
         finish_ab(a, weight, shift, s, u);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            float n = v[0][j] * inv;
+            float n = v[j] * inv;
             if (present & kNormA) n *= s[j];
             if (present & kNormB) n += u[j];
-            v[0][j] = n;
+            v[j] = n;
         }
     }
-    store_h(p, row, vec, in, v[0]);
+    store_h(p, row, vec, in, v);
 }
 
 // ------------------------------------------------------------------------------------------------ single elements
@@ -765,7 +756,7 @@ __device__ __forceinline__ float normalise_elements(float (&v)[NE], const NormPa
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < NE; ++i) s += v[i];
-        const float mean = row_sum<false>(s, part, flip) * p.inv_cols;
+        const float mean = row_sum(s, part, flip) * p.inv_cols;
 #pragma unroll
         for (int i = 0; i < NE; ++i)
             if (32 * i < left) v[i] -= mean;
@@ -773,7 +764,7 @@ __device__ __forceinline__ float normalise_elements(float (&v)[NE], const NormPa
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < NE; ++i) s += v[i] * v[i];
-    return 1.0f / sqrtf(row_sum<false>(s, part, flip) * p.inv_cols + p.a.eps);
+    return 1.0f / sqrtf(row_sum(s, part, flip) * p.inv_cols + p.a.eps);
 }
 
 // EARLY: what makes r is loaded together, what makes h of it before the second norm's sums; otherwise each where it is used.  48 registers there
