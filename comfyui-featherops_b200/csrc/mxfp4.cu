@@ -17,7 +17,7 @@ namespace feather {
 
 constexpr int kMxThreads = 256;
 
-// Rows of a thread where there are rows enough: loads under way against registers.  One, two, four and eight rows take 54, 49, 50, 71 us to
+// Rows of a thread where there are rows enough (eight elements a lane): loads under way against registers.  One, two, four and eight rows take 54, 49, 50, 71 us to
 // quantise 13824 x 5120 fp32 (48 us now, 6.7 TB/s, a copy's rate) and 36, 31, 30, 33 us for 4096 x 13824 bf16; dequantising 4096 x 13824 bf16 33, 26, 25, 25 us and 13824 x 5120 fp32 70,
 // 69, 72, 74 us (the rate at which memory is written).
 __host__ __device__ constexpr int mx_many_rows(int type) { return type == FEATHER_SRC_FP32 ? 2 : 4; }
@@ -210,30 +210,21 @@ static int mx_check(int64_t rows, int64_t K) {
 // (tx, ty) and grid: the narrowest power of two that covers a row's vectors, at most a whole block, and less where that leaves over a
 // sixteenth of the lanes idle (8192 x 5120 bf16: 21.7 -> 17.2 us).  *many: rows enough for threads of many_rows rows, whose grid still
 // fills the SMs twice over.
-static void mx_grid(int64_t rows, int64_t K, int elements, int many_rows, bool vector, dim3* grid, dim3* block, bool* many) {
+static void mx_grid(int64_t rows, int64_t K, int elements, int many_rows, bool vector, int sms, dim3* grid, dim3* block, bool* many) {
     const int64_t lanes = K / elements;
     unsigned tx = 128 / elements;
     while (tx < kMxThreads && tx < lanes) tx <<= 1;
     while (tx > 32 && ((lanes + tx - 1) / tx * tx - lanes) * 16 > lanes) tx >>= 1;
     const unsigned ty = kMxThreads / tx, along = static_cast<unsigned>((lanes + tx - 1) / tx);
-    *many = vector && (rows + ty * many_rows - 1) / (ty * many_rows) * along >= 2 * 148 * 8;
+    *many = vector && (rows + ty * many_rows - 1) / (ty * many_rows) * along >= 2 * sms * 8;
     const unsigned step = *many ? ty * many_rows : ty;
     *block = dim3(tx, ty, 1);
     *grid = dim3(static_cast<unsigned>((rows + step - 1) / step), along, 1);
 }
 
 template <typename... Params, typename... Args>
-static int mx_launch(const char* what, void (*kernel)(Params...), dim3 grid, dim3 block, cudaStream_t stream, Args... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+static int mx_launch(const char* what, void (*kernel)(Params...), dim3 grid, dim3 block, cudaStream_t stream, const Args&... args) {
+    const cudaError_t e = launch_dependent(kernel, grid, block, 0, 0, stream, args...);
     if (e != cudaSuccess) return set_error(FEATHER_ERR_CUDA, "%s launch failed: %s", what, cudaGetErrorString(e));
     return FEATHER_OK;
 }
@@ -269,17 +260,19 @@ extern "C" int feather_mxfp4_quantize(const void* src, int src_dtype, int64_t ro
     const int size = src_dtype == FEATHER_SRC_FP32 ? 4 : 2;
     if (reinterpret_cast<uintptr_t>(src) % size != 0) return set_error(FEATHER_ERR_BAD_ARGUMENT, "src must be aligned to its element size");
     const bool vector = mx_aligned16(src) && (rows == 1 || ld * size % 16 == 0);
+    const int sms = sm_count();
+    if (sms < 1) return set_error(FEATHER_ERR_CUDA, "the number of SMs could not be read");
     dim3 grid, block;
     bool many;
     const int k = static_cast<int>(K);
     const long long r = rows, l = ld;
     if (size == 2 && reinterpret_cast<uintptr_t>(src) % 32 == 0 && (rows == 1 || ld % 16 == 0)) {
-        mx_grid(rows, K, 16, 1, true, &grid, &block, &many);
+        mx_grid(rows, K, 16, 1, true, sms, &grid, &block, &many);
         const uint16_t* const s = static_cast<const uint16_t*>(src);
         return src_dtype == FEATHER_SRC_BF16 ? mx_launch("mxfp4_quantize", mx_quantize16_kernel<FEATHER_SRC_BF16>, grid, block, stream, s, r, k, l, data, scales)
                                              : mx_launch("mxfp4_quantize", mx_quantize16_kernel<FEATHER_SRC_FP16>, grid, block, stream, s, r, k, l, data, scales);
     }
-    mx_grid(rows, K, 8, mx_many_rows(src_dtype), vector, &grid, &block, &many);
+    mx_grid(rows, K, 8, mx_many_rows(src_dtype), vector, sms, &grid, &block, &many);
     switch (src_dtype) {
         case FEATHER_SRC_FP32: return mx_launch_quantize<FEATHER_SRC_FP32>(many, vector, grid, block, stream, src, r, k, l, data, scales);
         case FEATHER_SRC_BF16: return mx_launch_quantize<FEATHER_SRC_BF16>(many, vector, grid, block, stream, src, r, k, l, data, scales);
@@ -295,9 +288,11 @@ extern "C" int feather_mxfp4_dequantize(const uint8_t* data, const uint8_t* scal
     if (rows == 0) return FEATHER_OK;
     if (dst == nullptr || data == nullptr || scales == nullptr) return set_error(FEATHER_ERR_BAD_ARGUMENT, "data, scales and dst must not be null");
     if (!mx_aligned16(data) || !mx_aligned16(scales) || !mx_aligned16(dst)) return set_error(FEATHER_ERR_BAD_ARGUMENT, "data, scales and dst must be 16-byte aligned");
+    const int sms = sm_count();
+    if (sms < 1) return set_error(FEATHER_ERR_CUDA, "the number of SMs could not be read");
     dim3 grid, block;
     bool many;
-    mx_grid(rows, K, 8, mx_many_rows(dst_dtype), true, &grid, &block, &many);
+    mx_grid(rows, K, 8, mx_many_rows(dst_dtype), true, sms, &grid, &block, &many);
     const int k = static_cast<int>(K);
     const long long r = rows;
     switch (dst_dtype) {

@@ -23,8 +23,6 @@
 #include <stdint.h>
 #include <string.h>
 
-#include <mutex>
-
 #include "../../include/feather_b200.h"
 #include "host_util.h"
 #include "mxfp4.cuh"
@@ -56,11 +54,6 @@ __device__ __forceinline__ bool elect_one() {
         "}\n"
         : "=r"(p));
     return p != 0;
-}
-
-// Contiguous bytes global -> shared (both 16-byte aligned, size a multiple of 16), completion on an mbarrier.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
 // 32 rows x 16 bytes of shared memory -> 32 lanes x 4 columns of tensor memory, repeated in all four lane quarters.  The pair form
@@ -799,50 +792,6 @@ static CUresult mx_output_map(MxEncodeFn encode, CUtensorMap* out, void* c, int6
                   CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
-static int mx_sm_count() {
-    static std::mutex mu;
-    static int cached[64];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-    std::lock_guard<std::mutex> lock(mu);
-    if (cached[dev] == 0 && cudaDeviceGetAttribute(&cached[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-    return cached[dev];
-}
-
-// Opt-in shared memory of a kernel, once per device.
-template <typename Kernel>
-static cudaError_t mx_configure(Kernel kernel, int smem, bool (&configured)[64], std::mutex& mu) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    std::lock_guard<std::mutex> lock(mu);
-    if (configured[dev]) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    configured[dev] = e == cudaSuccess;
-    return e;
-}
-
-template <typename... Params, typename... Args>
-static cudaError_t mx_launch_cluster(void (*kernel)(Params...), long long ctas, int threads, int cluster, int smem, cudaStream_t stream, Args&... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
-    cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    // the CTAs may become resident and set up while the previous kernel on the stream drains; see pdl_wait_for_previous_kernel
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 // Features of a pair tile, by the time that its waves take.  Nanoseconds of a stage (256 k) and of a tile around its stages, fitted to
 // 8192 x 13824 x 5120 and 8192 x 5120 x 13824: 128 features 261 / 252 us, 192: 221 / 216, 256: 215 / 200 (the widest tile loads the least
 // and has the one accumulator that is read out between tiles).  Where few tiles leave pairs idle the narrower ones win:
@@ -865,13 +814,12 @@ static int mx_pair_features(int64_t M, int64_t N, int stages, int pairs) {
 template <int TF>
 static cudaError_t mx_launch_pair(const MxPairMaps& maps, const MxPairParams& p, int sms, cudaStream_t stream) {
     using C = MxPairCfg<TF>;
-    static std::mutex mu;
-    static bool configured[64];
-    cudaError_t e = mx_configure(mx_mm_pair_kernel<TF>, C::kSmemBytes, configured, mu);
+    static SmemOptIn opt_in;
+    cudaError_t e = opt_in(mx_mm_pair_kernel<TF>, C::kSmemBytes);
     if (e != cudaSuccess) return e;
     const long long tiles = static_cast<long long>(p.tiles_m) * p.tiles_n;
     const long long clusters = tiles < sms / 2 ? tiles : sms / 2;
-    return mx_launch_cluster(mx_mm_pair_kernel<TF>, clusters * 2, kMxPairThreads, 2, C::kSmemBytes, stream, maps, p);
+    return launch_dependent(mx_mm_pair_kernel<TF>, dim3(static_cast<unsigned>(clusters * 2)), dim3(kMxPairThreads), 2, C::kSmemBytes, stream, maps, p);
 }
 
 // K splits of a small product: the largest of 1, 2, 3, 4, 6 with which all CTAs are resident at once (two to an SM up to 32 tokens).
@@ -880,16 +828,15 @@ static cudaError_t mx_launch_pair(const MxPairMaps& maps, const MxPairParams& p,
 template <int TN>
 static cudaError_t mx_launch_mm(const CUtensorMap& tw, const CUtensorMap& tt, const MxMmParams& p, int sms, cudaStream_t stream) {
     using C = MxCfg<TN>;
-    static std::mutex mu;
-    static bool configured[64];
-    cudaError_t e = mx_configure(mx_mm_kernel<TN>, C::kSmemBytes, configured, mu);
+    static SmemOptIn opt_in;
+    cudaError_t e = opt_in(mx_mm_kernel<TN>, C::kSmemBytes);
     if (e != cudaSuccess) return e;
     const long long tiles = (p.N + kMxRows - 1) / kMxRows;
     int splits = 1;
     for (int s : {2, 3, 4, kMxMaxSplits})
         if (s <= p.stages_total && tiles * s <= static_cast<long long>(sms) * C::kPerSm) splits = s;
     const long long ctas = tiles * splits;
-    return mx_launch_cluster(mx_mm_kernel<TN>, ctas, kMxMmThreads, splits, C::kSmemBytes, stream, tw, tt, p, splits);
+    return launch_dependent(mx_mm_kernel<TN>, dim3(static_cast<unsigned>(ctas)), dim3(kMxMmThreads), splits, C::kSmemBytes, stream, tw, tt, p, splits);
 }
 
 }  // namespace feather
@@ -912,7 +859,7 @@ extern "C" int feather_mxfp4_mm(const uint8_t* a, const uint8_t* a_scales, const
     MxEncodeFn encode = mx_encode_fn();
     if (encode == nullptr) return set_error(FEATHER_ERR_NO_DEVICE, "cuTensorMapEncodeTiled is not available from the driver");
 
-    const int sms = mx_sm_count();
+    const int sms = sm_count();
     if (sms < 2) return set_error(FEATHER_ERR_CUDA, "the number of SMs could not be read");
     const int stages = static_cast<int>((K + kMxStageK - 1) / kMxStageK);
     cudaError_t e;

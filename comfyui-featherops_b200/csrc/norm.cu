@@ -12,7 +12,6 @@
 #include <stdint.h>
 #include <stdlib.h>
 
-#include <mutex>
 #include <type_traits>
 
 #include "../../include/feather_b200.h"
@@ -21,11 +20,6 @@
 #include "ptx.cuh"
 
 namespace feather {
-
-// Contiguous bytes global -> shared (both 16-byte aligned, size a multiple of 16), completion on an mbarrier.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
-}
 
 // Two fp32 values an instruction.
 struct F2 {
@@ -825,16 +819,6 @@ __global__ void __launch_bounds__(EARLY ? 256 : 1024, EARLY ? 5 : 1) gated_norm_
 }
 
 // ------------------------------------------------------------------------------------------------ launches
-static int norm_sm_count() {
-    static std::mutex mu;
-    static int cached[64];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-    std::lock_guard<std::mutex> lock(mu);
-    if (cached[dev] == 0 && cudaDeviceGetAttribute(&cached[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-    return cached[dev];
-}
-
 // Limit of a wait for a row of the ring: two seconds, or what FEATHER_NORM_WAIT_NS says if that is less (0: a row that is not there at the
 // first look counts as lost, which is how giving up is tested).
 static uint64_t norm_wait_ns() {
@@ -848,58 +832,15 @@ static uint64_t norm_wait_ns() {
 
 constexpr int kNormMaxSmem = 225 * 1024;      // dynamic, beside the sums and barriers
 
-template <typename... Params, typename... Args>
-static cudaError_t norm_launch_kernel(void (*kernel)(Params...), long long grid, int threads, int smem, cudaStream_t stream, const Args&... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
-    cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
-// How often a kernel is resident on an SM with this much shared memory, remembered by key.
-struct NormOccupancy {
-    std::mutex mu;
-    int blocks[64][256] = {};
-    template <typename Kernel>
-    cudaError_t get(Kernel kernel, int key, int threads, int smem, int* out) {
-        int dev = 0;
-        cudaError_t e = cudaGetDevice(&dev);
-        if (e != cudaSuccess) return e;
-        if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-        std::lock_guard<std::mutex> lock(mu);
-        int& known = blocks[dev][key];
-        if (known == 0) {
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormMaxSmem);
-            if (e != cudaSuccess) return e;
-            int n = 0;
-            e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem);
-            if (e != cudaSuccess) return e;
-            if (n < 1) return cudaErrorInvalidConfiguration;
-            known = n;
-        }
-        *out = known;
-        return cudaSuccess;
-    }
-};
-
-// Consecutive rows of each resident block.
-static int norm_chunk(int64_t rows, int64_t units) { return static_cast<int>((rows + units - 1) / units); }
-
+// One block an SM: its groups take the registers, its ring the shared memory. A block has consecutive rows.
 template <int XT, int YT, int NV, bool KEEP, bool FULL, bool POST>
 static cudaError_t norm_launch_groups_kernel(NormParams p, int threads, int smem, int sms, cudaStream_t stream) {
-    static NormOccupancy occupancy;
-    int blocks;
-    const cudaError_t e = occupancy.get(gated_norm_groups_kernel<XT, YT, NV, KEEP, FULL, POST>, smem / 1024, threads * p.groups, smem, &blocks);
+    static SmemOptIn opt_in;
+    const cudaError_t e = opt_in(gated_norm_groups_kernel<XT, YT, NV, KEEP, FULL, POST>, kNormMaxSmem);
     if (e != cudaSuccess) return e;
-    p.chunk = norm_chunk(p.a.rows, static_cast<int64_t>(blocks) * sms);
-    return norm_launch_kernel(gated_norm_groups_kernel<XT, YT, NV, KEEP, FULL, POST>, (p.a.rows + p.chunk - 1) / p.chunk, threads * p.groups, smem, stream, p);
+    p.chunk = static_cast<int>((p.a.rows + sms - 1) / sms);
+    return launch_dependent(gated_norm_groups_kernel<XT, YT, NV, KEEP, FULL, POST>, dim3(static_cast<unsigned>((p.a.rows + p.chunk - 1) / p.chunk)),
+                            dim3(static_cast<unsigned>(threads * p.groups)), 0, smem, stream, p);
 }
 
 template <int XT, int YT>
@@ -912,7 +853,7 @@ static cudaError_t norm_launch_groups(NormParams p, int sms, bool shared, cudaSt
     const int threads = (p.vecs + 32 * NV - 1) / (32 * NV) * 32;
     const int row_bytes = norm_row_bytes<XT, YT>(p.a);
     const int kept = norm_present(p.a) != 0 ? 3 * 32 * p.vecs : 0;
-    // One block an SM.  As many groups as its registers hold, each with two rows of ring at least; the coefficients stay in shared memory
+    // As many groups as its registers hold, each with two rows of ring at least; the coefficients stay in shared memory
     // if one group's row fits beside them.
     const bool keep = shared && kept + row_bytes <= kNormMaxSmem;
     const int room = kNormMaxSmem - (keep ? kept : 0);
@@ -942,10 +883,12 @@ static cudaError_t norm_launch_typed(const NormParams& p, int sms, cudaStream_t 
     if (a.shift != nullptr && a.shift_rows < shared) shared = a.shift_rows;
     // A block for each row up to two waves of them (16 of narrow rows: 2080 x 1024 fp32 7.8 us against 8.6 us, 1000 x 5120 27 us against 17 us),
     // and where every row has a modulation of its own.
-    if (p.vecs <= 1024 && (shared < 4 || a.rows <= (p.vecs <= 128 ? 16 : 2) * sms))
+    if (p.vecs <= 1024 && (shared < 4 || a.rows <= (p.vecs <= 128 ? 16 : 2) * sms)) {
+        const dim3 grid(static_cast<unsigned>(a.rows)), block((p.vecs + 31) / 32 * 32);
         return a.rows > 2 * sms && p.vecs > 512
-                   ? norm_launch_kernel(gated_norm_row_kernel<XT, YT, true>, a.rows, (p.vecs + 31) / 32 * 32, 0, stream, p)
-                   : norm_launch_kernel(gated_norm_row_kernel<XT, YT, false>, a.rows, (p.vecs + 31) / 32 * 32, 0, stream, p);
+                   ? launch_dependent(gated_norm_row_kernel<XT, YT, true>, grid, block, 0, 0, stream, p)
+                   : launch_dependent(gated_norm_row_kernel<XT, YT, false>, grid, block, 0, 0, stream, p);
+    }
     if (p.vecs <= 32) return norm_launch_groups<XT, YT, 1, true>(p, sms, shared >= 4, stream);
     if (p.vecs <= 64) return norm_launch_groups<XT, YT, 2, true>(p, sms, shared >= 4, stream);
     // The form without a norm of y, for the pairs of types that models have; it has its coefficients in shared memory always, and above 1536
@@ -1032,13 +975,14 @@ extern "C" int feather_gated_norm(const feather_norm_args* args_host, feather_st
     p.inv_cols = 1.0f / static_cast<float>(a.cols);
     p.wait_ns = norm_wait_ns();
     p.vecs = static_cast<int>(vector ? a.cols / 8 : a.cols);
-    const int sms = norm_sm_count();
+    const int sms = sm_count();
     if (sms < 1) return set_error(FEATHER_ERR_CUDA, "the number of SMs could not be read");
     cudaError_t e;
-    const auto threads = [&](int n) { return (p.vecs + 32 * n - 1) / (32 * n) * 32; };
+    const dim3 grid(static_cast<unsigned>(a.rows));
+    const auto block = [&](int n) { return dim3((p.vecs + 32 * n - 1) / (32 * n) * 32); };
     if (vector) e = norm_launch(p, sms, stream);
-    else if (p.vecs <= 2048) e = norm_launch_kernel(gated_norm_elements_kernel<8, true>, a.rows, threads(8), 0, stream, p);
-    else e = norm_launch_kernel(gated_norm_elements_kernel<16, false>, a.rows, threads(16), 0, stream, p);
+    else if (p.vecs <= 2048) e = launch_dependent(gated_norm_elements_kernel<8, true>, grid, block(8), 0, 0, stream, p);
+    else e = launch_dependent(gated_norm_elements_kernel<16, false>, grid, block(16), 0, 0, stream, p);
     if (e != cudaSuccess) return set_error(FEATHER_ERR_CUDA, "gated_norm launch failed: %s", cudaGetErrorString(e));
     return FEATHER_OK;
 }

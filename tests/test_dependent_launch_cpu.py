@@ -20,5 +20,5 @@ def _code(name):
 def test_no_read_only_loads(name):
     code = _code(name)
     if name.endswith(".cu"):
-        assert "cudaLaunchAttributeProgrammaticStreamSerialization" in code and "pdl_wait_for_previous_kernel" in code
+        assert "launch_dependent(" in code and "pdl_wait_for_previous_kernel" in code
     assert not re.findall(r"__ldg|\.nc\b|__restrict__", code)
