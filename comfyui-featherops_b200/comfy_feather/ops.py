@@ -53,13 +53,17 @@ class _FeatherLinear:
             missing_keys.append(prefix + "weight")
         else:
             self.is_quantized = not self._keeps_plain_weight(prefix, weight)
-            if self.is_quantized:
-                scale = weight_scale if weight_scale is not None else legacy_scale
-                weight = make_feather_quantized_weight(weight, scale, self.out_dtype)
-            elif self.in_features % 16 != 0:
-                print(f"Warning: Not prepacked {prefix}weight {tuple(weight.shape)}")
-            self.weight = _frozen(weight)
+            scale = weight_scale if weight_scale is not None else legacy_scale
+            self.weight = _frozen(self._quantized_weight(weight, scale) if self.is_quantized else self._plain_weight(prefix, weight, scale))
         self.bias = None if bias is None else _frozen(bias.to(self.out_dtype))
+
+    def _quantized_weight(self, weight, scale):
+        return make_feather_quantized_weight(weight, scale, self.out_dtype)
+
+    def _plain_weight(self, prefix, weight, scale):
+        if self.in_features % 16 != 0:
+            print(f"Warning: Not prepacked {prefix}weight {tuple(weight.shape)}")
+        return weight
 
     def convert_weight(self, weight, inplace=False, **kwargs):
         """The weight a LoRA merge works on: the dequantised matrix of a quantised layer."""
@@ -144,24 +148,15 @@ class _FeatherMXFP4Linear(_FeatherLinear):
     def _keeps_plain_weight(self, prefix, weight):
         return super()._keeps_plain_weight(prefix, weight) or self.in_features % 32 != 0
 
-    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
-        weight, bias, weight_scale, legacy_scale = (state_dict.pop(prefix + key, None) for key in _STATE_KEYS)
-        if weight is None:
-            missing_keys.append(prefix + "weight")
-        else:
-            self.is_quantized = not self._keeps_plain_weight(prefix, weight)
-            scale = weight_scale if weight_scale is not None else legacy_scale
-            if self.is_quantized:
-                weight = make_mxfp4_weight(weight, scale, self.out_dtype)
-            elif weight.dtype == torch.uint8:                      # MXFP4 in the checkpoint, excluded here
-                weight = make_mxfp4_weight(weight, scale, self.out_dtype).dequantize()
-            else:
-                if self.in_features % 32 != 0:
-                    print(f"Warning: Not MXFP4 {prefix}weight {tuple(weight.shape)}")
-                if scale is not None:
-                    weight = scaled_weight(weight, scale).to(self.out_dtype)
-            self.weight = _frozen(weight)
-        self.bias = None if bias is None else _frozen(bias.to(self.out_dtype))
+    def _quantized_weight(self, weight, scale):
+        return make_mxfp4_weight(weight, scale, self.out_dtype)
+
+    def _plain_weight(self, prefix, weight, scale):
+        if weight.dtype == torch.uint8:                            # MXFP4 in the checkpoint, excluded here
+            return make_mxfp4_weight(weight, scale, self.out_dtype).dequantize()
+        if self.in_features % 32 != 0:
+            print(f"Warning: Not MXFP4 {prefix}weight {tuple(weight.shape)}")
+        return weight if scale is None else scaled_weight(weight, scale).to(self.out_dtype)
 
     def convert_weight(self, weight, inplace=False, **kwargs):
         if self.is_quantized and not is_mxfp4_weight(weight):
