@@ -685,7 +685,7 @@ scaled_mm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
         const int grp = warp >> 2;
         const bool group_leader = (threadIdx.x & 127) == 0;
         const uint32_t t_lane = static_cast<uint32_t>(q * 32) << 16;
-        const float scale = (p.scale != nullptr ? __ldg(p.scale) : 1.0f) * (EXT ? p.scale_mul : 1.0f);
+        const float scale = (p.scale != nullptr ? *p.scale : 1.0f) * (EXT ? p.scale_mul : 1.0f);
         const bool out_bf16 = p.out_bf16 != 0;
         const bool flip = p.flip_final != 0;
         const bool has_bias = p.bias != nullptr;
@@ -713,13 +713,13 @@ scaled_mm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
             const int col = static_cast<int>(rank) * kBW + col_local;             // column inside the tile
             const int n = w.n0 + col;
             const bool n_ok = n < p.N;
-            const uint16_t bias_bits = (has_bias && n_ok) ? __ldg(reinterpret_cast<const uint16_t*>(p.bias) + n) : uint16_t(0);
+            const uint16_t bias_bits = (has_bias && n_ok) ? reinterpret_cast<const uint16_t*>(p.bias)[n] : uint16_t(0);
             // the staged path's fragment layout: this thread's four output columns (one per matrix), bias duplicated into both halves of a word
             uint32_t bias2[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int nn = w.n0 + static_cast<int>(rank) * kBW + q * 32 + 8 * i + (lane >> 2);
-                const uint32_t bb = (has_bias && nn < p.N) ? __ldg(reinterpret_cast<const uint16_t*>(p.bias) + nn) : 0u;
+                const uint32_t bb = (has_bias && nn < p.N) ? reinterpret_cast<const uint16_t*>(p.bias)[nn] : 0u;
                 bias2[i] = bb * 0x00010001u;
             }
             if (alive) {

@@ -17,7 +17,8 @@
 //               share a work item, each over 1/ks of K; a CTA parks its fp32 partial in the caller's workspace and the last
 //               of the ks to arrive (a counter per item) adds the partials in slice order - deterministic - and finishes
 //   launch      with programmatic dependent launch: the CTAs may become resident and run their prologue while the previous
-//               kernel on the stream drains; nothing touches global memory before griddepcontrol.wait
+//               kernel on the stream drains; nothing touches global memory before griddepcontrol.wait, and what is read
+//               is read by ordinary loads (the read-only path asks for memory that nobody writes during the kernel's life)
 //
 // Same math as kernel/hip/hip_kernel.cu:125-420 of the reference (which has no small-M path: its README.md:31 names an
 // unshipped split-k branch).
@@ -100,8 +101,8 @@ __device__ __forceinline__ uint16_t sm_finish(float acc, float scale, int out_mo
 // multiplied with every token group.  P: strips of 16 n per item.
 template <int P, int U, int NT>
 __global__ void __launch_bounds__(kSmThreads, 1)
-small_m8_kernel(const uint16_t* __restrict__ a, const uint8_t* __restrict__ w, const float* __restrict__ scale_ptr,
-                const uint16_t* __restrict__ bias, uint16_t* __restrict__ c, int M, int N, int K, long long ldc, int out_bf16, int num_items,
+small_m8_kernel(const uint16_t* a, const uint8_t* w, const float* scale_ptr,
+                const uint16_t* bias, uint16_t* c, int M, int N, int K, long long ldc, int out_bf16, int num_items,
                 SplitArgs sp) {
     constexpr int kCols = P * 16;
     constexpr int kPitch = kCols + 1;
@@ -114,7 +115,7 @@ small_m8_kernel(const uint16_t* __restrict__ a, const uint8_t* __restrict__ w, c
     const int nkb = K / 16;
     pdl_launch_dependents();
     pdl_wait_for_previous_kernel();
-    const float scale = scale_ptr != nullptr ? __ldg(scale_ptr) : 1.0f;
+    const float scale = scale_ptr != nullptr ? *scale_ptr : 1.0f;
     const bool has_bias = bias != nullptr;
 
     for (int item = blockIdx.x; item < num_items; item += gridDim.x) {
@@ -143,13 +144,13 @@ small_m8_kernel(const uint16_t* __restrict__ a, const uint8_t* __restrict__ w, c
 #pragma unroll
                 for (int s = 0; s < P; ++s) {
                     const int n0 = n_base + s * 16 + g;
-                    wv[u][s][0] = (kb_ok && n0 < N) ? __ldg(reinterpret_cast<const uint32_t*>(w_lane + kb * plane + s * 256)) : 0u;
-                    wv[u][s][1] = (kb_ok && n0 + 8 < N) ? __ldg(reinterpret_cast<const uint32_t*>(w_lane + kb * plane + s * 256 + 128)) : 0u;
+                    wv[u][s][0] = (kb_ok && n0 < N) ? *reinterpret_cast<const uint32_t*>(w_lane + kb * plane + s * 256) : 0u;
+                    wv[u][s][1] = (kb_ok && n0 + 8 < N) ? *reinterpret_cast<const uint32_t*>(w_lane + kb * plane + s * 256 + 128) : 0u;
                 }
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
                     tk[u][t] = (kb_ok && g + 8 * t < M)
-                                   ? __ldg(reinterpret_cast<const uint2*>(a + (g + 8 * t) * static_cast<long long>(K) + static_cast<long long>(kb) * 16 + 4 * j))
+                                   ? *reinterpret_cast<const uint2*>(a + (g + 8 * t) * static_cast<long long>(K) + static_cast<long long>(kb) * 16 + 4 * j)
                                    : make_uint2(0u, 0u);
             }
         };
@@ -199,7 +200,7 @@ small_m8_kernel(const uint16_t* __restrict__ a, const uint8_t* __restrict__ w, c
         auto emit = [&](int tok, int col, float sum) {
             const int n = n_base + col;
             if (tok < M && n < N) {
-                const uint16_t bias_bits = has_bias ? __ldg(bias + n) : uint16_t(0);
+                const uint16_t bias_bits = has_bias ? bias[n] : uint16_t(0);
                 c[static_cast<long long>(tok) * ldc + n] = sm_finish(sum, scale, out_bf16, has_bias, bias_bits);
             }
         };

@@ -16,9 +16,9 @@ def _code(name):
     return re.sub(r"//[^\n]*|/\*.*?\*/", "", text, flags=re.S)
 
 
-@pytest.mark.parametrize("name", ["mxfp4.cu", "mxfp4.cuh", "mxfp4_mm.cu", "norm.cu"])
+@pytest.mark.parametrize("name", ["mxfp4.cu", "mxfp4.cuh", "mxfp4_mm.cu", "norm.cu", "small_m.cu", "scaled_mm.cu"])
 def test_no_read_only_loads(name):
     code = _code(name)
     if name.endswith(".cu"):
-        assert "launch_dependent(" in code and "pdl_wait_for_previous_kernel" in code
+        assert ("launch_dependent(" in code or "ProgrammaticStreamSerialization" in code) and "pdl_wait_for_previous_kernel" in code
     assert not re.findall(r"__ldg|\.nc\b|__restrict__", code)
