@@ -4,7 +4,9 @@
 // the read-only path asks for memory that nobody writes during the kernel's life.
 //
 // Both are byte movers.  A lane holds eight elements, four lanes a block of 32 (16 and two for aligned 16-bit sources), so the block's
-// maximum is a shuffle or two and all loads and stores are whole vectors; nothing is staged and every byte is touched once.
+// maximum is a shuffle or two and all loads and stores are whole vectors; nothing is staged and every byte is touched once.  Rows that do not
+// begin on 16 bytes are loaded element by element: 4096 x 13824 bf16 40 us, 13824 x 5120 fp32 77 us (24 and 48 us aligned; bf16 rows on 16
+// bytes only, eight elements a lane, 32 us).
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -17,9 +19,10 @@ namespace feather {
 
 constexpr int kMxThreads = 256;
 
-// Rows of a thread where there are rows enough (eight elements a lane): loads under way against registers.  One, two, four and eight rows take 54, 49, 50, 71 us to
-// quantise 13824 x 5120 fp32 (48 us now, 6.7 TB/s, a copy's rate) and 36, 31, 30, 33 us for 4096 x 13824 bf16; dequantising 4096 x 13824 bf16 33, 26, 25, 25 us and 13824 x 5120 fp32 70,
-// 69, 72, 74 us (the rate at which memory is written).
+// Rows of a thread of the eight-element forms where there are rows enough: loads under way against registers.  One, two, four and eight rows take
+// 54, 49, 50, 71 us to quantise 13824 x 5120 fp32 (48 us now, 6.7 TB/s, a copy's rate) and 36, 31, 30, 33 us for 4096 x 13824 bf16 that is aligned to
+// 16 bytes only; dequantising 4096 x 13824 to bf16 33, 26, 25, 25 us and 13824 x 5120 to fp32 70, 69, 72, 74 us.  What bounds the last is not the
+// memory: a plain fill of its 283 MB takes 40 us, one of the 113 MB of the bf16 case 17 us; 82 % of the issue slots are used.
 __host__ __device__ constexpr int mx_many_rows(int type) { return type == FEATHER_SRC_FP32 ? 2 : 4; }
 
 // Eight elements as they lie in memory; 16-bit ones two to a word.  kVector: p is 16-byte aligned.

@@ -296,8 +296,9 @@ __device__ __forceinline__ void join8(const float (&f)[8], F2 (&v)[4]) {
 // lie in shared memory, once for the block, and are folded anew where a wave begins that belongs to other rows of gate, scale or shift
 // (a wave ends there).
 // Bound by the instructions around the arithmetic rather than by memory: 2 x 8192 x 5120 bf16 with fp32 gate, scale and shift of each
-// sample takes 127 us as layer norm (5.3 TB/s of 671 MB), 154 us as a packed result, 185 us with a norm of y before it; a block for each
-// row that reads its vectors from the cache takes 213 us for the first.
+// sample takes 128 us as layer norm (5.2 TB/s of 671 MB), 156 us as a packed result, 185 us with a norm of y before it; a block for each
+// row that reads its vectors from the cache takes 213 us for the first.  Leaving the loop when a wait runs out costs the first 1 us and the
+// packed one 3 us (the vote after the wait); a flag that the rows test instead cost up to 10 us, and 20 us at 256 columns.
 constexpr int kNormMaxStages = 4, kNormMaxGroups = 32, kNormMaxBarriers = 15;    // a group of one warp needs no barrier
 // Registers of a thread.  POST: y may go through a norm first, and x has to wait for it in registers.  Without that norm r is formed as x
 // and y are read, 96 registers are enough, and rows of 5120 have four groups instead of three (127 us where 128 registers take 141).

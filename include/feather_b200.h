@@ -300,6 +300,8 @@ FEATHER_API int feather_mxfp4_mm(const uint8_t* a, const uint8_t* a_scales, cons
  * row i / gate_rows (scale_rows, shift_rows) belongs to row i of x, with row pitch gate_ld (scale_ld, shift_ld).
  * With h_scales, h is MXFP4 data (ldh is ignored): the bits of feather_mxfp4_quantize over the h of type h_dtype.  That needs
  * cols % 32 == 0 and 16-byte aligned rows everywhere.  cols is at most 16384.  r and h must not overlap an input.
+ * A wait that runs out (two seconds, or FEATHER_NORM_WAIT_NS nanoseconds if that is less) is recorded in *status_dev; what would have
+ * been made of the row is then NaN or not written.
  * ------------------------------------------------------------------------------------------- */
 enum { FEATHER_NORM_RMS = 0, FEATHER_NORM_LAYER = 1 };
 typedef struct feather_norm_args {
