@@ -21,7 +21,8 @@ import torch
 from .b200 import native
 
 
-SCALE_DTYPES = (torch.uint8, torch.float8_e8m0fnu)                          # what E8M0 bytes are stored as
+# What E8M0 bytes are stored as; older torch has no type for them.
+SCALE_DTYPES = tuple(getattr(torch, name) for name in ("uint8", "float8_e8m0fnu") if hasattr(torch, name))
 
 
 def _tiles(rows, k):

@@ -1,6 +1,7 @@
 """CPU: what the MXFP4 Linear makes of a checkpoint's weight and scale where no kernel is needed."""
 
 import importlib
+import importlib.util
 
 import pytest
 import torch
@@ -95,3 +96,14 @@ def test_a_packed_weight_that_lies_unaligned_is_copied(pkg):
         weight = layout.make_mxfp4_weight(view, scale, torch.bfloat16)
         assert weight._qdata.data_ptr() % 16 == 0 and weight._qdata.is_contiguous() and torch.equal(weight._qdata, view)
         assert (weight._qdata.data_ptr() == view.data_ptr()) == (offset % 16 == 0)       # no copy where none is needed
+
+
+def test_a_torch_without_the_e8m0_type_still_imports(pkg, monkeypatch):
+    """The fp8 operators import this module too."""
+    mx = importlib.import_module("feather_b200.kernel.mxfp4")
+    monkeypatch.delattr(torch, "float8_e8m0fnu")
+    spec = importlib.util.spec_from_file_location("feather_b200.kernel.mxfp4_again", mx.__file__)
+    source = open(mx.__file__).read().split("# ---", 1)[0]                   # up to the operators, which register once
+    space = {"__name__": spec.name, "__package__": "feather_b200.kernel"}
+    exec(compile(source, mx.__file__, "exec"), space)
+    assert space["SCALE_DTYPES"] == (torch.uint8,)
