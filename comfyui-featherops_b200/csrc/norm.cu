@@ -825,7 +825,9 @@ __global__ void __launch_bounds__(EARLY ? 256 : 1024, EARLY ? 5 : 1) gated_norm_
 static uint64_t norm_wait_ns() {
     static const uint64_t ns = [] {
         const char* const text = getenv("FEATHER_NORM_WAIT_NS");
-        const unsigned long long asked = text != nullptr ? strtoull(text, nullptr, 10) : kWaitLimitNs;
+        char* rest = nullptr;
+        const unsigned long long asked = text != nullptr ? strtoull(text, &rest, 10) : 0;
+        if (text == nullptr || rest == text || *rest != '\0') return kWaitLimitNs;             // unset, or not a number
         return asked < kWaitLimitNs ? static_cast<uint64_t>(asked) : kWaitLimitNs;
     }();
     return ns;

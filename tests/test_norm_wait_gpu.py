@@ -76,6 +76,15 @@ def call(native, case, status):
     return outs
 
 
+@pytest.mark.parametrize("limit", ["", "soon", "5 s", "-1", "99999999999999999999"])
+def test_a_limit_that_is_no_shorter_number_is_the_default(pkg, native, cuda_dev, tmp_path, limit):
+    script, out = tmp_path / "wait.py", tmp_path / "seen.pt"
+    script.write_text(SCRIPT % ROOT)
+    res = subprocess.run([sys.executable, str(script), str(out)], env={**os.environ, "FEATHER_NORM_WAIT_NS": limit}, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=180, cwd=ROOT)
+    assert res.returncode == 0, res.stdout[-3000:]
+    assert all(code == 0 for code, _ in torch.load(out))
+
+
 def test_a_wait_that_runs_out(pkg, native, cuda_dev, tmp_path):
     script, out = tmp_path / "wait.py", tmp_path / "seen.pt"
     script.write_text(SCRIPT % ROOT)
