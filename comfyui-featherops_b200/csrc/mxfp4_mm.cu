@@ -129,7 +129,9 @@ __device__ __forceinline__ float load16(const uint16_t* p, bool bf16) {
 __device__ __forceinline__ uint16_t round16(float v, bool bf16) { return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v)); }
 
 // Up to this many tokens the weights are on the lanes and K is split over a cluster: 64 x 13824 x 5120 takes 11.9 us this way and 13.9 us
-// on CTA pairs, 128 x 13824 x 5120 15.8 us (with 128-token tiles) and 13.9 us.
+// on CTA pairs, 128 x 13824 x 5120 15.8 us (with 128-token tiles) and 13.9 us.  17 and 64 x 5120 x 13824: 11.2 and 12.7 us against 23.0 and 16.9;
+// 17 and 64 x 5120 x 5120: 8.0 and 8.8 against 11.1 and 9.2.  Where K is short the border lies lower: 32 and 64 x 1024 x 1024 4.0 and 5.8 against 4.7
+// and 4.8, 32 and 64 x 2811 x 1056 5.2 and 6.5 against 6.3 and 6.4.
 constexpr int kMxSmallTokens = 64;
 constexpr int kMxRows = 128;                        // weight rows of a tile: the lanes
 constexpr int kMxMmThreads = 192;                   // producer warp, MMA warp, four epilogue warps

@@ -885,7 +885,9 @@ static cudaError_t norm_launch_typed(const NormParams& p, int sms, cudaStream_t 
     if (a.scale != nullptr && a.scale_rows < shared) shared = a.scale_rows;
     if (a.shift != nullptr && a.shift_rows < shared) shared = a.shift_rows;
     // A block for each row up to two waves of them (16 of narrow rows: 2080 x 1024 fp32 7.8 us against 8.6 us, 1000 x 5120 27 us against 17 us),
-    // and where every row has a modulation of its own.
+    // and where every row has a modulation of its own.  bf16 with a norm of y, a block a row against groups: 600 x 256 3.2 and 6.5 us, 2368 x 512 5.8
+    // and 6.5, 4800 x 512 10.7 and 9.0; 600 x 1024 4.7 and 6.1, but 1200 x 1024 7.1 and 6.4; 300 x 2048 4.8 and 6.6, 600 x 2048 7.3 and 7.0; 150 x 5120
+    // 7.8 and 7.8, 300 x 5120 10.2 and 8.8.
     if (p.vecs <= 1024 && (shared < 4 || a.rows <= (p.vecs <= 128 ? 16 : 2) * sms)) {
         const dim3 grid(static_cast<unsigned>(a.rows)), block((p.vecs + 31) / 32 * 32);
         return a.rows > 2 * sms && p.vecs > 512
