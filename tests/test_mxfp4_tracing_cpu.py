@@ -89,3 +89,21 @@ def test_export(block):
         args = _inputs()
     program = torch.export.export(Module(), args, strict=False)
     assert _count([n.target for n in program.graph.nodes if n.op == "call_function"]) == NAMES
+
+
+def test_compile_takes_the_whole_block(block):
+    """One graph without a break; it is only looked at here, not run."""
+    graphs = []
+
+    class Seen(Exception):
+        pass
+
+    def backend(gm, example_inputs):
+        graphs.append(gm)
+        raise Seen
+
+    torch._dynamo.reset()
+    with pytest.raises(Exception, match="Seen"):
+        torch.compile(block, backend=backend, fullgraph=True)(*_inputs("cpu"))
+    assert _count([getattr(n.target, "_opoverload", n.target) for n in graphs[0].graph.nodes if n.op == "call_function"]) == NAMES
+    torch._dynamo.reset()

@@ -29,7 +29,7 @@ def _block(mx, norm, b, sb):
     return run
 
 
-@pytest.mark.parametrize("how", ["jit", "fx", "fx_pre_dispatch", "fx_symbolic"])
+@pytest.mark.parametrize("how", ["jit", "fx", "fx_pre_dispatch", "fx_symbolic", "compile_eager", "compile_aot_eager"])
 def test_traced(fns, cuda_dev, how):
     mx, norm = fns
     g = torch.Generator().manual_seed(1)
@@ -41,9 +41,12 @@ def test_traced(fns, cuda_dev, how):
     first, second = inputs(70), inputs(70)
     if how == "jit":
         traced = torch.jit.trace(run, first)
+    elif how.startswith("compile"):
+        torch._dynamo.reset()
+        traced = torch.compile(run, backend=how[len("compile_"):], fullgraph=True)
     else:
         traced = make_fx(run, pre_dispatch=how == "fx_pre_dispatch", tracing_mode="symbolic" if how == "fx_symbolic" else "real", _allow_non_fake_inputs=True)(*first)
-    for args in (first, second) + ((inputs(9),) if how == "fx_symbolic" else ()):
+    for args in (first, second) + ((inputs(9),) if how == "fx_symbolic" or how.startswith("compile") else ()):
         for got, want in zip(traced(*args), run(*args)):
             assert torch.equal(got.view(torch.int16), want.view(torch.int16))
 
